@@ -46,6 +46,12 @@ extern "C" {
 #define ONN_DELTA_READY        16u     /* Dense backward: dY already holds dY * act'(Y) */
 #define ONN_CE_TWO_SWEEPS      32u     /* onn_ce3d_fwd_bwd: keep to the kernel that sweeps each row twice through global memory */
 
+/* element types of logits (onn_token_logprobs, onn_distill3d_fwd_bwd); what is computed from them is held in fp32 */
+#define ONN_F32   0
+#define ONN_BF16  1
+#define ONN_F16   2
+#define ONN_TOP_MAX 128                /* most alternatives / teacher's tokens of a row */
+
 /* activations of Dense<3> used by the transformer (opennn/standard_networks.cpp:745,753,890) */
 #define ONN_ACT_LINEAR   0
 #define ONN_ACT_RELU     1
@@ -184,6 +190,17 @@ int onn_ids_to_float(const int32_t* ids, float* out, int64_t n, void* stream);
  * dY2 may be NULL. */
 int onn_embedding_bwd(const float* ids, const float* dY, const float* dY2, float* dW,
                       int64_t B, int64_t S, int64_t E, int64_t V, int scale, void* stream);
+
+/* The same gradient summed by token in a fixed order, for callers that want the same bits from every run:
+ *   dW[v,:] = sqrt(E) (if scale) * sum over the positions with id v, in order of position, of (dY + dY2),  0 < v < V.
+ * Nothing is added atomically, so frequent tokens do not contend (onn_embedding_bwd adds each position's row with
+ * fp32 reductions in whatever order they arrive).  flags 0: all of dW [V, E] is overwritten, with zeros for
+ * row 0 and for tokens that do not occur; ONN_ACCUMULATE: added to the rows of the tokens that do, the others are left
+ * alone.  E, V < 2^24, B * S < 2^31.  workspace: onn_embedding_bwd_sorted_workspace_floats floats (may be NULL when that is 0). */
+size_t onn_embedding_bwd_sorted_workspace_floats(int64_t B, int64_t S, int64_t E, int64_t V);
+int onn_embedding_bwd_sorted(const float* ids, const float* dY, const float* dY2, float* dW,
+                             int64_t B, int64_t S, int64_t E, int64_t V, int scale,
+                             float* workspace, uint32_t flags, void* stream);
 
 /* ---------------------------------------------------------------------------------------
  * Normalization3d (LayerNorm over the last dimension) with the preceding Addition<3> fused.
@@ -372,6 +389,62 @@ int onn_ce3d_fwd_bwd(float* logits, const float* targets, const float* active_co
                      float* probabilities_out, float* stats, float* row_scratch,
                      int64_t rows, int64_t V, int inputs_are_probabilities,
                      uint32_t flags, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Log probabilities of given tokens, with entropy and the top alternatives (no counterpart in the reference, whose
+ * only reader of the distribution is the arg-max of its decoding loop, opennn/standard_networks.cpp:1016-1034).
+ * For each row of logits [rows, V] (element type dtype = ONN_F32 / ONN_BF16 / ONN_F16, row r at logits + r * pitch
+ * elements, pitch >= V, any alignment), with z = logits / temperature:
+ *   lse      = log sum exp z
+ *   logprob  = z[token] - lse
+ *   entropy  = -sum p log p,  p = exp(z - lse)
+ *   top      the `top` <= ONN_TOP_MAX largest logits in falling order, equal ones in order of index: index and z - lse.
+ * logprobs, entropy, lse are [rows]; top_ids, top_logprobs [rows, top].  Each may be NULL (top_ids and top_logprobs
+ * only with top = 0) but not all; all are fp32 / int32 whatever dtype is.
+ * tokens (floats holding integers, [rows]): a row whose token is not in (0, V) is padding, as in onn_ce3d_fwd_bwd; it is
+ * not read and receives 0, 0, 0 and a list of -1 with -inf.  NULL: every row takes part, and logprobs must be NULL.
+ * Logits of -inf (masked tokens) have probability 0 and never stand in the list; places left over hold -1 and -inf.
+ * A row of nothing but -inf receives -inf, 0, -inf and an empty list.  A row that holds NaN or +inf receives NaN
+ * for logprob, entropy and lse and in the values of its list (NaN logits are not listed).
+ * temperature is in [1e-6, 1e6]; rows < 2^27.
+ * ------------------------------------------------------------------------------------- */
+int onn_token_logprobs(const void* logits, int dtype, int64_t pitch, const float* tokens,
+                       float* logprobs, float* entropy, float* lse, int32_t* top_ids, float* top_logprobs, int64_t top,
+                       int64_t rows, int64_t V, float temperature, void* stream);
+/* Its gradient with respect to the logits: with lse and entropy [rows] as onn_token_logprobs wrote them and the
+ * gradients of the two outputs, d_logprobs [rows] and d_entropy [rows] (NULL: no gradient through the entropy; entropy
+ * may then be NULL too),
+ *   dlogits_i = (d_logprob (1[i = token] - p_i) - d_entropy p_i (log p_i + entropy)) / temperature,
+ * 0 on padding rows, rounded once to dtype.  dlogits (row r at dlogits + r * d_pitch elements) is overwritten; it may
+ * be the logits themselves (same pitch), but must not overlap them in another way.  Elements between V and the pitch
+ * are left as they are. */
+int onn_token_logprobs_bwd(const void* logits, int dtype, int64_t pitch, const float* tokens, const float* lse,
+                           const float* entropy, const float* d_logprobs, const float* d_entropy,
+                           void* dlogits, int64_t d_pitch, int64_t rows, int64_t V, float temperature, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Distillation from a teacher's top logits, beside onn_ce3d_fwd_bwd (no counterpart in the reference): the loss of a
+ * student's logits [rows, V] against a list of `top` <= ONN_TOP_MAX tokens per row -- what onn_token_logprobs lists for
+ * a teacher -- mixed with CrossEntropyError3d's hard-label loss, and its gradient, in one call.
+ * teacher_ids, teacher_logits [rows, top]: token index and logit or log probability (any constant added to a row's
+ * values cancels); a place whose id is outside [0, V) is unused; an id may stand in several places.  Per active row
+ * (0 < (integer) target < V), with T = temperature:
+ *   q    = softmax over the valid places of teacher_logits / T;  p = softmax(logits / T);  p1 = softmax(logits)
+ *   soft = T^2 sum q (log q - log p[id])                 (0 where no place is valid; q = 0 adds 0)
+ *   hard = -log(p1[target] + FLT_EPSILON)                (not computed, 0, when hard_weight is 0)
+ *   dlogits = [soft_weight T (p - q) + hard_weight (p1 - onehot)] / active_count[0]
+ * (the soft part is 0 where no place is valid) and 0 on the other rows, rounded once to dtype.
+ * row_losses [2 * rows] receives soft, then hard, of each row (0 on inactive ones); stats (device, 3 floats) receives
+ * {sum of soft, sum of hard, #active (local)}.  active_count (device): as in onn_ce3d_fwd_bwd; NULL = the #active of
+ * this call.  logits, dtype, pitch, temperature as in onn_token_logprobs; dlogits as in onn_token_logprobs_bwd: it may
+ * be the logits themselves, and NULL computes the losses alone.  A logit of -inf has p = 0, and makes soft (hard)
+ * +inf (-log FLT_EPSILON) where a teacher's token (the target) is masked; NaN and +inf make the row NaN.
+ * ------------------------------------------------------------------------------------- */
+int onn_distill3d_fwd_bwd(const void* logits, int dtype, int64_t pitch, const float* targets, const float* active_count,
+                          const int32_t* teacher_ids, const float* teacher_logits, int64_t top,
+                          float temperature, float soft_weight, float hard_weight,
+                          void* dlogits, int64_t d_pitch, float* stats, float* row_losses,
+                          int64_t rows, int64_t V, void* stream);
 
 /* CrossEntropyError2d with several classes (the loss of the text-classification network).  Replaces
  * calculate_multiple_cross_entropy_cuda + the gradient kernel (opennn/cross_entropy_error.cpp:217-300); CPU semantics

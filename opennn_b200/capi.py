@@ -53,7 +53,9 @@ class MhaGrads(C.Structure):
 
 EXPORTS = [
     "onn_status_string", "onn_version", "onn_gemm", "onn_gemm_set_mode", "onn_mha_set_kv_grad_by_recomputation", "onn_gemm_device_status",
-    "onn_launch_count", "onn_launch_count_add", "onn_selftest_bounded_wait", "onn_embedding_fwd", "onn_embedding_bwd", "onn_ids_to_float",
+    "onn_launch_count", "onn_launch_count_add", "onn_selftest_bounded_wait", "onn_embedding_fwd", "onn_embedding_bwd",
+    "onn_embedding_bwd_sorted_workspace_floats", "onn_embedding_bwd_sorted", "onn_token_logprobs", "onn_token_logprobs_bwd",
+    "onn_distill3d_fwd_bwd", "onn_ids_to_float",
     "onn_layernorm_fwd", "onn_layernorm_bwd_workspace_floats", "onn_layernorm_bwd", "onn_layernorm_bwd_static", "onn_add",
     "onn_relu_bits_words_per_row", "onn_dense_fwd", "onn_dense_bwd", "onn_pooling3d_fwd", "onn_pooling3d_bwd", "onn_softmax_rows",
     "onn_mha_fwd_workspace_floats", "onn_mha_bwd_workspace_floats", "onn_mha_fwd", "onn_mha_bwd",
@@ -81,6 +83,14 @@ def lib():
             getattr(L, name).restype = C.c_size_t
             getattr(L, name).argtypes = None
         L.onn_mha_attention_weights.restype = C.c_void_p
+        # declared argument types: addresses and sizes go across as plain Python numbers (None = NULL)
+        p, n, f = C.c_void_p, C.c_int64, C.c_float
+        L.onn_token_logprobs.argtypes = [p, C.c_int, n, p, p, p, p, p, p, n, n, n, f, p]
+        L.onn_token_logprobs_bwd.argtypes = [p, C.c_int, n, p, p, p, p, p, p, n, n, n, f, p]
+        L.onn_distill3d_fwd_bwd.argtypes = [p, C.c_int, n, p, p, p, p, n, f, f, f, p, n, p, p, n, n, p]
+        L.onn_embedding_bwd_sorted_workspace_floats.argtypes = [n, n, n, n]
+        L.onn_embedding_bwd_sorted_workspace_floats.restype = C.c_size_t
+        L.onn_embedding_bwd_sorted.argtypes = [p, p, p, p, n, n, n, n, C.c_int, p, C.c_uint32, p]
         _lib = L
     return _lib
 
@@ -157,6 +167,47 @@ def embedding_bwd(ids, dY, V, scale=True, dY2=None):
     dW = torch.zeros(V, E, device="cuda")
     check(lib().onn_embedding_bwd(ptr(ids), ptr(dY), ptr(dY2), ptr(dW), i64(B), i64(S), i64(E), i64(V), int(scale),
                                   stream_ptr()), "onn_embedding_bwd")
+    return dW
+
+
+def _f32(t, shape, what):
+    """Address of a float tensor of a given shape (None = NULL)."""
+    if t is None:
+        return None
+    if t.dtype is not torch.float32 or t.numel() != shape or not t.is_cuda or not t.is_contiguous():
+        raise OnnError(f"{what}: a contiguous float32 device tensor of {shape} elements is needed")
+    return t.data_ptr()
+
+
+def _i32(t, shape, what):
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.numel() != shape or not t.is_cuda or not t.is_contiguous():
+        raise OnnError(f"{what}: a contiguous int32 device tensor of {shape} elements is needed")
+    return t.data_ptr()
+
+
+def _current_stream(t):
+    """The current stream, which has to be one of the device that holds t."""
+    stream = torch.cuda.current_stream()
+    if t.get_device() != stream.device_index:
+        raise OnnError(f"the tensors are on cuda:{t.get_device()}, the current device is cuda:{stream.device_index}")
+    return stream.cuda_stream
+
+
+def embedding_bwd_sorted(ids, dY, V, scale=True, dY2=None, dW=None, accumulate=False):
+    """embedding_bwd with the rows of each token added in order of position.  dW [V, E] is written (a new tensor if None),
+    or added to with accumulate=True."""
+    B, S, E = dY.shape
+    if dW is None:
+        dW = (torch.zeros if accumulate else torch.empty)(V, E, device="cuda")
+    L = lib()
+    n = B * S
+    stream = _current_stream(dY)
+    workspace = _empty(L.onn_embedding_bwd_sorted_workspace_floats(B, S, E, V))
+    check(L.onn_embedding_bwd_sorted(_f32(ids, n, "ids"), _f32(dY, n * E, "dY"), _f32(dY2, n * E, "dY2"), _f32(dW, V * E, "dW"),
+                                     B, S, E, V, int(scale), workspace.data_ptr(), ACCUMULATE if accumulate else 0, stream),
+          "onn_embedding_bwd_sorted")
     return dW
 
 
@@ -306,6 +357,91 @@ def ce3d(logits, targets, inputs_are_probabilities=False, want_probabilities=Fal
     error = loss_sum / active if active > 0 else 0.0
     accuracy = correct / active if active > 0 else 0.0
     return error, accuracy, logits, probabilities
+
+
+LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _logit_rows(t, what):
+    """(address, type, row pitch, rows, V) of logits [..., V] whose elements are adjacent and whose rows are evenly spaced."""
+    dtype = LOGIT_TYPES.get(t.dtype)
+    if dtype is None or not t.is_cuda or t.dim() < 1:
+        raise OnnError(f"{what}: a float32, bfloat16 or float16 device tensor [..., V] is needed")
+    shape = t.shape
+    V = shape[-1]
+    if t.dim() == 2:
+        rows, (pitch, inner) = shape[0], t.stride()
+        if rows == 1:
+            pitch = V
+    else:
+        rows, stride = t.numel() // V if V else 0, t.stride()
+        inner, pitch, spaced = stride[-1], V, None
+        for size, step in zip(shape[-2::-1], stride[-2::-1]):
+            if size == 1:
+                continue
+            if spaced is None:
+                pitch = step
+            elif step != spaced:
+                raise OnnError(f"{what}: the rows must be evenly spaced")
+            spaced = step * size
+    if inner != 1 and V != 1:
+        raise OnnError(f"{what}: the elements of a row must be adjacent")
+    return t.data_ptr(), dtype, pitch, rows, V
+
+
+def token_logprobs(logits, tokens=None, top=0, temperature=1.0, out=None):
+    """Log probabilities of `tokens` (floats holding integers, one per row; rows of padding receive zeros) under logits
+    [..., V] in float32, bfloat16 or float16.  Returns (logprobs, entropy, lse, top_ids, top_logprobs): fp32 [rows], the lists
+    [rows, top] in int32 and fp32; logprobs is None without tokens, the lists with top=0.  out: a tuple as returned,
+    to be written again."""
+    x, dtype, pitch, rows, V = _logit_rows(logits, "logits")
+    stream = _current_stream(logits)
+    if out is None:
+        out = (None if tokens is None else _empty(rows), _empty(rows), _empty(rows),
+               torch.empty(rows, top, dtype=torch.int32, device="cuda") if top > 0 else None,
+               torch.empty(rows, top, device="cuda") if top > 0 else None)
+    logprobs, entropy, lse, top_ids, top_logprobs = out
+    check(lib().onn_token_logprobs(x, dtype, pitch, _f32(tokens, rows, "tokens"), _f32(logprobs, rows, "logprobs"),
+                                   _f32(entropy, rows, "entropy"), _f32(lse, rows, "lse"), _i32(top_ids, rows * top, "top_ids"),
+                                   _f32(top_logprobs, rows * top, "top_logprobs"), top, rows, V, temperature, stream), "onn_token_logprobs")
+    return out
+
+
+def token_logprobs_bwd(logits, tokens, lse, entropy, d_logprobs, d_entropy=None, temperature=1.0, out=None):
+    """The gradient of token_logprobs' logprobs and entropy with respect to the logits.  out may be the logits themselves."""
+    x, dtype, pitch, rows, V = _logit_rows(logits, "logits")
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    dx, d_dtype, d_pitch, d_rows, d_V = _logit_rows(out, "out")
+    if (d_dtype, d_rows, d_V) != (dtype, rows, V):
+        raise OnnError("out: the logits' shape and type are needed")
+    check(lib().onn_token_logprobs_bwd(x, dtype, pitch, _f32(tokens, rows, "tokens"), _f32(lse, rows, "lse"),
+                                       _f32(entropy, rows, "entropy"), _f32(d_logprobs, rows, "d_logprobs"),
+                                       _f32(d_entropy, rows, "d_entropy"), dx, d_pitch, rows, V, temperature,
+                                       _current_stream(logits)), "onn_token_logprobs_bwd")
+    return out
+
+
+def distill3d(logits, targets, teacher_ids, teacher_logits, temperature=1.0, soft_weight=1.0, hard_weight=0.0, active_count=None,
+              want_gradient=True, out=None):
+    """Distillation from a teacher's top logits (teacher_ids int32, teacher_logits fp32, [rows, top]) mixed with the hard-label
+    loss.  Returns (stats {sum of soft, sum of hard, #active}, row losses [2, rows], gradient or None), all on the device.
+    out: a tuple as returned, to be written again; its gradient may be the logits themselves."""
+    x, dtype, pitch, rows, V = _logit_rows(logits, "logits")
+    top = teacher_ids.shape[-1]
+    if out is None:
+        out = (_empty(3), torch.empty(2, rows, device="cuda"),
+               torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if want_gradient else None)
+    stats, row_losses, gradient = out
+    dx, d_dtype, d_pitch, d_rows, d_V = (None, dtype, V, rows, V) if gradient is None else _logit_rows(gradient, "gradient")
+    if (d_dtype, d_rows, d_V) != (dtype, rows, V):
+        raise OnnError("gradient: the logits' shape and type are needed")
+    check(lib().onn_distill3d_fwd_bwd(x, dtype, pitch, _f32(targets, rows, "targets"), _f32(active_count, 1, "active_count"),
+                                      _i32(teacher_ids, rows * top, "teacher_ids"), _f32(teacher_logits, rows * top, "teacher_logits"),
+                                      top, temperature, soft_weight, hard_weight, dx, d_pitch, _f32(stats, 3, "stats"),
+                                      _f32(row_losses, 2 * rows, "row_losses"), rows, V, _current_stream(logits)),
+          "onn_distill3d_fwd_bwd")
+    return out
 
 
 def ce2d(probabilities, targets):

@@ -1,0 +1,134 @@
+// Rows of logits in fp32, bf16 or fp16: 16-byte vectors of a row and the elements around them, shared by the kernels
+// that read logits (token_logprobs.cu, distill.cu).
+//
+// A row starts wherever `pitch` puts it, so it is cut into up to VE - 1 leading elements, a body of 16-byte vectors that
+// starts on a 16-byte boundary, and up to VE - 1 trailing elements.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "common.cuh"
+#include "launch_counter.h"
+
+namespace onn
+{
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int DTYPE> struct Logit;
+
+template <> struct Logit<ONN_F32>
+{
+    using type = float;
+    static constexpr int VE = 4;                     // elements of a 16-byte vector
+    static __device__ __forceinline__ float get(const type* p) { return *p; }
+    static __device__ __forceinline__ void put(type* p, float v) { *p = v; }
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[VE])
+    {
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[VE])
+    {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+    static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xff800000u; return make_uint4(v, v, v, v); }
+};
+
+template <> struct Logit<ONN_BF16>
+{
+    using type = __nv_bfloat16;
+    static constexpr int VE = 8;
+    static __device__ __forceinline__ float get(const type* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ void put(type* p, float v) { *p = __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[VE])
+    {
+        const unsigned int w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for(int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[VE])
+    {
+        unsigned int w[4];
+#pragma unroll
+        for(int i = 0; i < 4; i++)
+        {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned int*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xff80ff80u; return make_uint4(v, v, v, v); }
+};
+
+template <> struct Logit<ONN_F16>
+{
+    using type = __half;
+    static constexpr int VE = 8;
+    static __device__ __forceinline__ float get(const type* p) { return __half2float(*p); }
+    static __device__ __forceinline__ void put(type* p, float v) { *p = __float2half_rn(v); }
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[VE])
+    {
+        const unsigned int w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for(int i = 0; i < 4; i++)
+        {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[VE])
+    {
+        unsigned int w[4];
+#pragma unroll
+        for(int i = 0; i < 4; i++)
+        {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned int*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xfc00fc00u; return make_uint4(v, v, v, v); }
+};
+
+// head + VE * vectors + tail = V; the body starts 16-byte aligned.
+struct RowCut { int head, vectors, tail; };
+
+template <int DTYPE>
+__device__ __forceinline__ RowCut cut_row(const void* row, int V)
+{
+    constexpr int VE = Logit<DTYPE>::VE;
+    RowCut c;
+    c.head = (int)((-reinterpret_cast<intptr_t>(row)) & 15) / (16 / VE);
+    if(c.head > V) c.head = V;
+    c.vectors = (V - c.head) / VE;
+    c.tail = V - c.head - c.vectors * VE;
+    return c;
+}
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A row takes part when its token is in (0, V): 0 is padding, as in the loss.  Without tokens every row does.
+__device__ __forceinline__ long long row_token(const float* tokens, long long row, int V, bool* active)
+{
+    if(!tokens) { *active = true; return -1; }
+    const long long t = token_index(__ldg(tokens + row));
+    *active = t > 0 && t < V;
+    return t;
+}
+
+inline int logit_bytes(int dtype) { return dtype == ONN_F32 ? 4 : 2; }
+inline bool logit_arguments_ok(const void* logits, int dtype, int64_t pitch, int64_t rows, int64_t V)
+{
+    return logits && dtype >= ONN_F32 && dtype <= ONN_F16 && V > 1 && V < (1LL << 31) - 4096 && pitch >= V &&
+           rows > 0 && rows < (1LL << 27) && reinterpret_cast<uintptr_t>(logits) % logit_bytes(dtype) == 0;
+}
+inline bool temperature_ok(float t) { return t > 0.f && t <= 1e6f && t >= 1e-6f; }
+
+}  // namespace onn
