@@ -33,6 +33,11 @@ template <> struct Logit<ONN_F32>
     {
         return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
     }
+    // the largest element; NaN is passed by (-inf for nothing but NaN)
+    static __device__ __forceinline__ float max(const uint4& v)
+    {
+        return fmaxf(-INFINITY, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+    }
     static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xff800000u; return make_uint4(v, v, v, v); }
 };
 
@@ -58,6 +63,12 @@ template <> struct Logit<ONN_BF16>
             w[i] = *reinterpret_cast<const unsigned int*>(&h);
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ float max(const uint4& v)
+    {
+        auto h = [](unsigned int w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+        const float2 f = __bfloat1622float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
+        return fmaxf(-INFINITY, fmaxf(f.x, f.y));
     }
     static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xff80ff80u; return make_uint4(v, v, v, v); }
 };
@@ -89,6 +100,12 @@ template <> struct Logit<ONN_F16>
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    static __device__ __forceinline__ float max(const uint4& v)
+    {
+        auto h = [](unsigned int w) { return *reinterpret_cast<const __half2*>(&w); };
+        const float2 f = __half22float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
+        return fmaxf(-INFINITY, fmaxf(f.x, f.y));
+    }
     static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xfc00fc00u; return make_uint4(v, v, v, v); }
 };
 
@@ -114,6 +131,38 @@ __device__ __forceinline__ float exp2_approx(float x)
     return y;
 }
 
+// Two fp32 operations per instruction.
+__device__ __forceinline__ unsigned long long pair_bits(float2 v)
+{
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 pair_of(unsigned long long r)
+{
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+    return v;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+    return pair_of(r);
+}
+
 // A row takes part when its token is in (0, V): 0 is padding, as in the loss.  Without tokens every row does.
 __device__ __forceinline__ long long row_token(const float* tokens, long long row, int V, bool* active)
 {
@@ -121,6 +170,24 @@ __device__ __forceinline__ long long row_token(const float* tokens, long long ro
     const long long t = token_index(__ldg(tokens + row));
     *active = t > 0 && t < V;
     return t;
+}
+
+// A launch in clusters of `ctas` CTAs.
+template <typename... KernelArgs, typename... Args>
+inline cudaError_t launch_clusters(void (*kernel)(KernelArgs...), unsigned int grid, int threads, int ctas, cudaStream_t stream, Args&&... args)
+{
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(threads);
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = ctas;
+    attribute[0].val.clusterDim.y = 1;
+    attribute[0].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
 }
 
 inline int logit_bytes(int dtype) { return dtype == ONN_F32 ? 4 : 2; }
