@@ -38,6 +38,8 @@ template <> struct Logit<ONN_F32>
     {
         return fmaxf(-INFINITY, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
     }
+    static constexpr bool floors = false;                // -inf stays: a sum that multiplies by it has to look
+    static __device__ __forceinline__ uint4 floor(const uint4& v) { return v; }
     static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xff800000u; return make_uint4(v, v, v, v); }
 };
 
@@ -69,6 +71,18 @@ template <> struct Logit<ONN_BF16>
         auto h = [](unsigned int w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
         const float2 f = __bfloat1622float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
         return fmaxf(-INFINITY, fmaxf(f.x, f.y));
+    }
+    // -inf (and anything below -1e30) as -1e30, NaN as it is: finite, and as far below any other logit as makes no difference
+    static constexpr bool floors = true;
+    static __device__ __forceinline__ uint4 floor(const uint4& v)
+    {
+        const unsigned int bound = 0xf14af14au;              // -1.0e30 twice
+        auto at_least = [&](unsigned int w)
+        {
+            const __nv_bfloat162 h = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&bound));
+            return *reinterpret_cast<const unsigned int*>(&h);
+        };
+        return make_uint4(at_least(v.x), at_least(v.y), at_least(v.z), at_least(v.w));
     }
     static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xff80ff80u; return make_uint4(v, v, v, v); }
 };
@@ -106,6 +120,8 @@ template <> struct Logit<ONN_F16>
         const float2 f = __half22float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
         return fmaxf(-INFINITY, fmaxf(f.x, f.y));
     }
+    static constexpr bool floors = false;                // -inf stays: a sum that multiplies by it has to look
+    static __device__ __forceinline__ uint4 floor(const uint4& v) { return v; }
     static __device__ __forceinline__ uint4 lowest() { const unsigned int v = 0xfc00fc00u; return make_uint4(v, v, v, v); }
 };
 

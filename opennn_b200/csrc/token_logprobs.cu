@@ -19,20 +19,24 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 8;                        // 16-byte vectors a thread has in flight
 
-// Running statistics of a set of logits, in base 2 and relative to the largest logit m seen: with c = log2(e) / T and
-// d = c (x - m),  s = sum 2^d  and  w = sum 2^d d.  The difference is taken before the scale, so logits of any finite
-// size (a mask of the type's lowest value) leave it finite or at -inf; -inf adds nothing to either sum; NaN and +inf
-// make both NaN.
+// Running statistics of a set of logits, in base 2 and relative to the largest logit m seen: with c = log2(e) / T,
+// a = c max(m, -kHuge) and d = c x - a in one rounding,  s = sum 2^d  and  w = sum 2^d d.  Every set with the
+// same m has the same a, so its rounding shifts all terms alike and is taken out at the end.  -inf adds nothing to either
+// sum; NaN and +inf make both NaN.  Logits below -kHuge count as nothing, and beyond |m| = kHuge c x could overflow: a row
+// whose largest logit is that far out is summed again (huge_row).
 struct Running { float m, s, w; };
 
 constexpr float kNothing = -1e4f;                 // 2^-10000 = 0: the bound that keeps 0 * -inf out of w
+constexpr float kHuge = 1e29f;
 
 __device__ __forceinline__ float finite_anchor(float m) { return m > -INFINITY ? m : 0.f; }
+// rounded once, whatever it is subtracted from (no contraction into a fused multiply-add)
+__device__ __forceinline__ float anchor(float m, float c) { return __fmul_rn(fmaxf(m, -kHuge), c); }
 
 // The sums of r relative to another, larger m.
 __device__ __forceinline__ void rebase(Running& r, float m, float c)
 {
-    const float d = fmaxf((r.m - finite_anchor(m)) * c, kNothing);
+    const float d = fmaxf(anchor(r.m, c) - anchor(m, c), kNothing);
     const float f = exp2_approx(d);
     r.w = fmaf(d, r.s, r.w) * f;
     r.s *= f;
@@ -49,32 +53,51 @@ __device__ __forceinline__ Running merge(Running a, Running b, float c)
     return a;
 }
 
-// Adds the logits of kUnroll vectors, of which the largest is `m`: one rescaling for all of them, then two logits per
-// instruction (packed fp32).
-template <int DTYPE>
-__device__ __forceinline__ void add_vectors(Running& r, const uint4 (&v)[kUnroll], float m, float c)
+// Adds the logits of N vectors, of which the largest (with those before) is `m`: one rescaling for all of them, then two
+// logits per instruction (packed fp32).
+template <int DTYPE, int N>
+__device__ __forceinline__ void add_vectors(Running& r, const uint4 (&v)[N], float m, float c)
 {
     using L = Logit<DTYPE>;
     if(m > r.m) rebase(r, m, c);
-    const float base = finite_anchor(r.m);
-    const float2 minus_base = make_float2(-base, -base), c2 = make_float2(c, c);
+    const float a = anchor(r.m, c);
+    const float2 minus_a = make_float2(-a, -a), c2 = make_float2(c, c);
     float2 s2 = make_float2(0.f, 0.f), w2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for(int u = 0; u < kUnroll; u++)
+    for(int u = 0; u < N; u++)
     {
         float x[L::VE];
-        L::unpack(v[u], x);
+        L::unpack(L::floor(v[u]), x);
 #pragma unroll
         for(int e = 0; e < L::VE; e += 2)
         {
-            const float2 d = mul2(add2(make_float2(x[e], x[e + 1]), minus_base), c2);
+            float2 d = fma2(make_float2(x[e], x[e + 1]), c2, minus_a);
             const float2 p = make_float2(exp2_approx(d.x), exp2_approx(d.y));
             s2 = add2(s2, p);
-            w2 = fma2(p, make_float2(fmaxf(d.x, kNothing), fmaxf(d.y, kNothing)), w2);
+            if(!L::floors) d = make_float2(fmaxf(d.x, kNothing), fmaxf(d.y, kNothing));
+            w2 = fma2(p, d, w2);
         }
     }
     r.s += s2.x + s2.y;
     r.w += w2.x + w2.y;
+}
+
+// The sums of a whole row by one warp, with the difference taken before the scale: right for logits of any finite size
+// (nothing but a mask of the type's lowest value), and rare.
+template <int DTYPE>
+__device__ __noinline__ Running huge_row(const typename Logit<DTYPE>::type* x, int V, float m, float c)
+{
+    Running r = {m, 0.f, 0.f};
+    for(int i = threadIdx.x & 31; i < V; i += 32)
+    {
+        const float d = (Logit<DTYPE>::get(x + i) - m) * c;
+        const float p = exp2_approx(d);
+        r.s += p;
+        r.w = fmaf(p, fmaxf(d, kNothing), r.w);
+    }
+    r.s = warp_sum(r.s);
+    r.w = warp_sum(r.w);
+    return r;
 }
 
 // Order of the alternatives as one number: the larger logit first, then the lower index.  0 = not in the list at all
@@ -93,26 +116,22 @@ __device__ __forceinline__ float key_logit(unsigned long long key)
     return __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// k-th largest of the lanes' values (k from 1 to 32): a bitonic sort across the warp.
-__device__ __forceinline__ float warp_kth_largest(float v, int k)
+// A value that at least k lanes reach (k from 1 to 32): the largest is taken away k times.  Equal ones go together, which
+// only lowers the result.
+__device__ __forceinline__ float warp_reached_by(float v, int k)
 {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for(int size = 2; size <= 32; size <<= 1)
+    float t;
+    while(true)
     {
-#pragma unroll
-        for(int stride = size >> 1; stride > 0; stride >>= 1)
-        {
-            const float other = __shfl_xor_sync(0xffffffffu, v, stride);
-            const bool falling = (lane & size) == 0 || size == 32, first = (lane & stride) == 0;
-            v = falling == first ? fmaxf(v, other) : fminf(v, other);
-        }
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(t) : "f"(v));
+        if(--k == 0) return t;
+        if(v == t) v = -INFINITY;
     }
-    return __shfl_sync(0xffffffffu, v, k - 1);
 }
 
 constexpr int kMaxCluster = 8;
-constexpr int kList = 2048;                       // candidates a CTA can hold
+constexpr int kHits = 1024;                       // vectors with a possible alternative that a CTA can hold
+constexpr int kCandidates = 1024;
 
 // What a warp knows of its part of the row.
 struct alignas(16) Part { float m, s, w, top; };
@@ -130,23 +149,24 @@ struct Shared<true>
     Part parts[kMaxCluster * kWarps];
     float m, log_s;
     volatile float warp_top[kWarps];
-    int listed, candidate_count;
+    int hits, candidate_count;
     unsigned long long best[kWarps];
-    unsigned long long list[kList];
-    unsigned long long candidates[kList];
+    uint4 hit[kHits];
+    int hit_index[kHits];
+    unsigned long long candidates[kCandidates];
 };
 
 // One cluster of CTAs (often of one) per row; each CTA streams its part of the row once.
 //
 // The alternatives come out of the same pass.  If every warp knows k logits that are at least t, with k = ceil(top /
-// warps), no logit below t can stand in the list.  So after its first batch every warp sorts its lanes' maxima and takes
-// the k-th as its bound; the smallest bound of all warps is the CTA's, and logits that reach it are put on a list in shared
-// memory (a compare per vector; for logits in no particular order a few hundred of them).  The bounds rise after 2, 4, 8 ... batches.  At
-// the end the bound of all maxima thins the lists out to little more than `top` candidates in the first CTA, which ranks
-// them.  A list that overflows (thousands of equal logits, a rising row) is done without: the first CTA then scans
-// the row once for each place.
-template <int DTYPE, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? 3 : 4)
+// warps), no logit below t can stand in the list.  So after its first batch every warp takes of its lanes' maxima
+// the k-th as its bound; the smallest bound of all warps is the CTA's, and vectors with a logit that reaches it are put on
+// a list in shared memory (a compare per vector; for logits in no particular order a few hundred of them).  The bounds
+// rise after 2, 3, 5, 9 ... batches.  At the end the bound of all maxima thins the lists out to little more than `top`
+// candidates in the first CTA, which ranks them.  A list that overflows (thousands of equal logits, a rising row) is done
+// without: the first CTA then scans the row once for each place.
+template <int DTYPE, bool TOP, int N>
+__global__ void __launch_bounds__(kThreads, 4)
 token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, long long pitch, const float* __restrict__ tokens,
                       float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ lse,
                       int* __restrict__ top_ids, float* __restrict__ top_logprobs, int top, int V, float c, float inverse_temperature)
@@ -186,22 +206,11 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
 
     if constexpr(TOP)
     {
-        if(tid == 0) { shared.listed = 0; shared.candidate_count = 0; }
+        if(tid == 0) { shared.hits = 0; shared.candidate_count = 0; }
     }
     // all CTAs of a cluster must be running before one writes into another
     if(ctas > 1) cluster.sync();
     else if constexpr(TOP) __syncthreads();
-
-    [[maybe_unused]] auto list_one = [&](float value, int index)
-    {
-        if constexpr(TOP)
-        {
-            const unsigned long long key = key_of(value, index);
-            if(key == 0) return;
-            const int at = atomicAdd(&shared.listed, 1);
-            if(at < kList) shared.list[at] = key;
-        }
-    };
 
     Running r = {-INFINITY, 0.f, 0.f};
     float end_value = -INFINITY;
@@ -210,51 +219,47 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         end_value = L::get(x + end_index);
         // as a batch of its own; NaN is never larger, and reaches the sum
         r.m = end_value > -INFINITY ? end_value : -INFINITY;
-        r.s = exp2_approx((end_value - finite_anchor(r.m)) * c);
+        r.s = exp2_approx(fmaf(end_value, c, -anchor(r.m, c)));
+        r.w = r.s * fmaxf(fmaf(end_value, c, -anchor(r.m, c)), kNothing);
     }
     const int wanted = TOP ? (top + kWarps - 1) / kWarps : 1;
     float bound = -INFINITY;
-    for(int first = begin, batch = 0; first < end || batch == 0; first += kThreads * kUnroll, batch++)
+    for(int first = begin, batch = 0; first < end || batch == 0; first += kThreads * N, batch++)
     {
-        uint4 v[kUnroll];
+        uint4 v[N];
 #pragma unroll
-        for(int u = 0; u < kUnroll; u++)
+        for(int u = 0; u < N; u++)
         {
             const int i = first + u * kThreads + tid;
             v[u] = i < end ? __ldg(body + i) : L::lowest();
         }
-        float vector_max[kUnroll];
+        float vector_max[N];
         float m = r.m;
 #pragma unroll
-        for(int u = 0; u < kUnroll; u++)
+        for(int u = 0; u < N; u++)
         {
             vector_max[u] = L::max(v[u]);
             m = fmaxf(m, vector_max[u]);
         }
-        add_vectors<DTYPE>(r, v, m, c);
+        add_vectors<DTYPE, N>(r, v, m, c);
         if constexpr(TOP)
         {
-            if((batch & (batch - 1)) == 0)             // after 1, 2, 3, 5, 9 ... batches
+            if((batch & (batch - 1)) == 0)             // batches 0, 1, 2, 4, 8 ...
             {
-                const float mine = warp_kth_largest(r.m, wanted);
+                const float mine = warp_reached_by(r.m, wanted);
                 if(lane == 0) shared.warp_top[warp] = mine;
                 // the first bound needs every warp's; later ones take what is there, since bounds only rise
                 if(batch == 0) __syncthreads();
                 bound = shared.warp_top[0];
 #pragma unroll
                 for(int w = 1; w < kWarps; w++) bound = fminf(bound, shared.warp_top[w]);
-                if(batch == 0 && end_value >= bound) list_one(end_value, end_index);
             }
 #pragma unroll
-            for(int u = 0; u < kUnroll; u++)
+            for(int u = 0; u < N; u++)
             {
                 if(vector_max[u] < bound || vector_max[u] == -INFINITY) continue;
-                float part[VE];
-                L::unpack(v[u], part);
-                const int index = cut.head + (first + u * kThreads + tid) * VE;
-#pragma unroll
-                for(int e = 0; e < VE; e++)
-                    if(part[e] >= bound) list_one(part[e], index + e);
+                const int at = atomicAdd(&shared.hits, 1);
+                if(at < kHits) { shared.hit[at] = v[u]; shared.hit_index[at] = cut.head + (first + u * kThreads + tid) * VE; }
             }
         }
     }
@@ -269,7 +274,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     part.w = warp_sum(r.w);
     const int parts = ctas * kWarps;
     const int wanted_all = TOP ? (top + parts - 1) / parts : 1;
-    part.top = TOP ? warp_kth_largest(own_max, wanted_all) : 0.f;
+    part.top = TOP ? warp_reached_by(own_max, wanted_all) : 0.f;
     if(ctas == 1)
     {
         if(lane == 0) shared.parts[warp] = part;
@@ -288,16 +293,20 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         rebase(all, warp_max(all.m), c);
         all.s = warp_sum(all.s);
         all.w = warp_sum(all.w);
+        const bool huge = fabsf(all.m) >= kHuge && fabsf(all.m) < INFINITY;
+        if(huge) all = huge_row<DTYPE>(x, V, all.m, c);
         if(lane == 0)
         {
             const bool none = all.s == 0.f;            // a row without a finite logit has no distribution
-            const float log_s = none ? INFINITY : logf(all.s);
+            const float log_2s = logf(all.s);
+            // relative to m itself: the rounding of the anchor
+            const float log_s = none ? INFINITY : huge ? log_2s : fmaf(fmaf(all.m, c, -anchor(all.m, c)), -kLn2, log_2s);
             shared.m = finite_anchor(all.m);
             shared.log_s = log_s;
             if(logprobs) logprobs[row] = none ? -INFINITY : (L::get(x + token) - all.m) * inverse_temperature - log_s;
             if(entropy)
             {
-                const float value = log_s - all.w / all.s * kLn2;
+                const float value = log_2s - all.w / all.s * kLn2;
                 entropy[row] = none || value < 0.f ? 0.f : value;
             }
             if(lse) lse[row] = none ? -INFINITY : fmaf(all.m, inverse_temperature, log_s);
@@ -326,20 +335,29 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             for(int i = lane; i < parts; i += 32) lowest = fminf(lowest, shared.parts[i].top);
             bound = -warp_max(-lowest);
         }
-        const int listed = shared.listed;
+        const int hits = shared.hits;
         Shared<TOP>* leader = ctas == 1 ? &shared : cluster.map_shared_rank(&shared, 0);
-        if(listed > kList)
+        auto candidate = [&](float value, int index)
         {
-            if(tid == 0) atomicAdd(&leader->candidate_count, kList + 1);
+            const unsigned long long key = key_of(value, index);
+            if(!(value >= bound) || key == 0) return;
+            const int at = atomicAdd(&leader->candidate_count, 1);
+            if(at < kCandidates) leader->candidates[at] = key;
+        };
+        if(hits > kHits)
+        {
+            if(tid == 0) atomicAdd(&leader->candidate_count, kCandidates + 1);
         }
         else
         {
-            for(int i = tid; i < listed; i += kThreads)
+            if(end_index >= 0) candidate(end_value, end_index);
+            for(int i = tid; i < hits; i += kThreads)
             {
-                const unsigned long long key = shared.list[i];
-                if(key_logit(key) < bound) continue;
-                const int at = atomicAdd(&leader->candidate_count, 1);
-                if(at < kList) leader->candidates[at] = key;
+                float values[VE];
+                L::unpack(shared.hit[i], values);
+                const int index = shared.hit_index[i];
+#pragma unroll
+                for(int e = 0; e < VE; e++) candidate(values[e], index + e);
             }
         }
         if(ctas == 1) __syncthreads();
@@ -352,7 +370,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             top_logprobs[row * top + k] = key ? (key_logit(key) - shared.m) * inverse_temperature - shared.log_s : -INFINITY;
         };
         int n = shared.candidate_count;
-        if(n < 0 || n > kList)
+        if(n > kCandidates)
         {
             // one place after the other: the largest key below the last one
             unsigned long long last = ~0ull;
@@ -400,6 +418,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             {
                 const unsigned long long key = shared.candidates[tid];
                 int larger = 0;
+#pragma unroll 4
                 for(int j = 0; j < n; j++) larger += shared.candidates[j] > key;
                 if(larger < top) place(larger, key);
             }
@@ -489,7 +508,7 @@ token_logprobs_bwd_kernel(const typename Logit<DTYPE>::type* logits, long long p
     }
 }
 
-template <int DTYPE, bool TOP>
+template <int DTYPE, bool TOP, int N>
 int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float* logprobs, float* entropy, float* lse,
                   int32_t* top_ids, float* top_logprobs, int64_t top, int64_t rows, int64_t V, float c, float inverse_temperature,
                   cudaStream_t stream)
@@ -498,7 +517,7 @@ int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float*
     // few rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read
     int ctas = 1;
     while(ctas < kMaxCluster && rows * ctas * 2 <= 4 * kSmCount && V / L::VE >= (int64_t)ctas * 2 * kThreads * 2) ctas *= 2;
-    if(launch_clusters(token_logprobs_kernel<DTYPE, TOP>, (unsigned)(rows * ctas), kThreads, ctas, stream,
+    if(launch_clusters(token_logprobs_kernel<DTYPE, TOP, N>, (unsigned)(rows * ctas), kThreads, ctas, stream,
                        static_cast<const typename L::type*>(logits), (long long)pitch, tokens, logprobs, entropy, lse, top_ids,
                        top_logprobs, (int)top, (int)V, c, inverse_temperature) != cudaSuccess) return ONN_ERR_CUDA;
     count_launch();
@@ -510,7 +529,8 @@ int launch_fwd(const void* logits, int64_t pitch, const float* tokens, float* lo
                int32_t* top_ids, float* top_logprobs, int64_t top, int64_t rows, int64_t V, float c, float inverse_temperature,
                cudaStream_t stream)
 {
-    const auto launch = top > 0 ? launch_fwd_as<DTYPE, true> : launch_fwd_as<DTYPE, false>;
+    constexpr int N = DTYPE == ONN_F32 ? 8 : 4;
+    const auto launch = top > 0 ? launch_fwd_as<DTYPE, true, N> : launch_fwd_as<DTYPE, false, N>;
     return launch(logits, pitch, tokens, logprobs, entropy, lse, top_ids, top_logprobs, top, rows, V, c, inverse_temperature, stream);
 }
 
