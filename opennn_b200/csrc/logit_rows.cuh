@@ -33,10 +33,10 @@ template <> struct Logit<ONN_F32>
     {
         return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
     }
-    // the largest element; NaN is passed by (-inf for nothing but NaN)
+    // the largest element; NaN is passed by (NaN for nothing but NaN)
     static __device__ __forceinline__ float max(const uint4& v)
     {
-        return fmaxf(-INFINITY, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
     }
     static constexpr bool floors = false;                // -inf stays: a sum that multiplies by it has to look
     static __device__ __forceinline__ uint4 floor(const uint4& v) { return v; }
@@ -70,7 +70,7 @@ template <> struct Logit<ONN_BF16>
     {
         auto h = [](unsigned int w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
         const float2 f = __bfloat1622float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
-        return fmaxf(-INFINITY, fmaxf(f.x, f.y));
+        return fmaxf(f.x, f.y);
     }
     // -inf (and anything below -1e30) as -1e30, NaN as it is: finite, and as far below any other logit as makes no difference
     static constexpr bool floors = true;
@@ -118,7 +118,7 @@ template <> struct Logit<ONN_F16>
     {
         auto h = [](unsigned int w) { return *reinterpret_cast<const __half2*>(&w); };
         const float2 f = __half22float2(__hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w))));
-        return fmaxf(-INFINITY, fmaxf(f.x, f.y));
+        return fmaxf(f.x, f.y);
     }
     static constexpr bool floors = false;                // -inf stays: a sum that multiplies by it has to look
     static __device__ __forceinline__ uint4 floor(const uint4& v) { return v; }

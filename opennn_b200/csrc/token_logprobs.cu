@@ -6,6 +6,9 @@
 //
 // Both are bound by HBM: the forward pass reads each logit once, the backward pass reads and writes each once.
 #include <cooperative_groups.h>
+#include <float.h>
+
+#include <type_traits>
 
 #include "logit_rows.cuh"
 
@@ -116,21 +119,21 @@ __device__ __forceinline__ float key_logit(unsigned long long key)
     return __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// A value that at least k lanes reach (k from 1 to 32): the largest is taken away k times.  Equal ones go together, which
-// only lowers the result.
-__device__ __forceinline__ float warp_reached_by(float v, int k)
+// A value that at least k of the lanes' pairs of logits (first >= second) reach: the largest is taken away k times.  Equal
+// ones of several lanes go together, which only lowers the result.
+__device__ __forceinline__ float warp_reached_by(float first, float second, int k)
 {
     float t;
     while(true)
     {
-        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(t) : "f"(v));
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(t) : "f"(first));
         if(--k == 0) return t;
-        if(v == t) v = -INFINITY;
+        if(first == t) { first = second; second = -INFINITY; }
     }
 }
 
 constexpr int kMaxCluster = 8;
-constexpr int kHits = 1024;                       // vectors with a possible alternative that a CTA can hold
+constexpr int kHits = 160;                        // vectors with a possible alternative that a warp can hold
 constexpr int kCandidates = 1024;
 
 // What a warp knows of its part of the row.
@@ -149,24 +152,24 @@ struct Shared<true>
     Part parts[kMaxCluster * kWarps];
     float m, log_s;
     volatile float warp_top[kWarps];
-    int hits, candidate_count;
+    int candidate_count;
     unsigned long long best[kWarps];
-    uint4 hit[kHits];
-    int hit_index[kHits];
+    uint4 hit[kWarps][kHits];
+    int hit_index[kWarps][kHits];
     unsigned long long candidates[kCandidates];
 };
 
 // One cluster of CTAs (often of one) per row; each CTA streams its part of the row once.
 //
 // The alternatives come out of the same pass.  If every warp knows k logits that are at least t, with k = ceil(top /
-// warps), no logit below t can stand in the list.  So after its first batch every warp takes of its lanes' maxima
-// the k-th as its bound; the smallest bound of all warps is the CTA's, and vectors with a logit that reaches it are put on
-// a list in shared memory (a compare per vector; for logits in no particular order a few hundred of them).  The bounds
-// rise after 2, 3, 5, 9 ... batches.  At the end the bound of all maxima thins the lists out to little more than `top`
-// candidates in the first CTA, which ranks them.  A list that overflows (thousands of equal logits, a rising row) is done
-// without: the first CTA then scans the row once for each place.
+// warps), no logit below t can stand in the list.  So after its first batch every warp takes the k-th largest of its
+// lanes' two best vectors as its bound; the smallest bound of all warps is the CTA's, and vectors with a logit that reaches
+// it go on the warp's list in shared memory (a compare per vector; for logits in no particular order a few hundred
+// of a row).  The bounds rise after 2, 3, 5, 9 ... batches.  At the end the bound of all warps thins the lists out to little
+// more than `top` candidates in the first CTA, which ranks them.  A list that overflows (a rising row) is replaced by
+// another scan with the final bound; candidates that overflow (a thousand equal logits) by a scan for each place.
 template <int DTYPE, bool TOP, int N>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, N > 4 && TOP ? 3 : 4)
 token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, long long pitch, const float* __restrict__ tokens,
                       float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ lse,
                       int* __restrict__ top_ids, float* __restrict__ top_logprobs, int top, int V, float c, float inverse_temperature)
@@ -206,7 +209,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
 
     if constexpr(TOP)
     {
-        if(tid == 0) { shared.hits = 0; shared.candidate_count = 0; }
+        if(tid == 0) shared.candidate_count = 0;
     }
     // all CTAs of a cluster must be running before one writes into another
     if(ctas > 1) cluster.sync();
@@ -223,15 +226,16 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         r.w = r.s * fmaxf(fmaf(end_value, c, -anchor(r.m, c)), kNothing);
     }
     const int wanted = TOP ? (top + kWarps - 1) / kWarps : 1;
-    float bound = -INFINITY;
-    for(int first = begin, batch = 0; first < end || batch == 0; first += kThreads * N, batch++)
+    [[maybe_unused]] float bound = -FLT_MAX, second = -INFINITY;     // of this lane's vectors, the second largest maximum
+    [[maybe_unused]] int hits = 0;                                   // on the warp's list
+    auto take = [&](const int first, const int batch, auto whole)
     {
         uint4 v[N];
 #pragma unroll
         for(int u = 0; u < N; u++)
         {
             const int i = first + u * kThreads + tid;
-            v[u] = i < end ? __ldg(body + i) : L::lowest();
+            v[u] = whole.value || i < end ? __ldg(body + i) : L::lowest();
         }
         float vector_max[N];
         float m = r.m;
@@ -239,6 +243,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         for(int u = 0; u < N; u++)
         {
             vector_max[u] = L::max(v[u]);
+            if constexpr(TOP) second = fmaxf(second, vector_max[u] > m ? m : vector_max[u]);       // NaN is passed by
             m = fmaxf(m, vector_max[u]);
         }
         add_vectors<DTYPE, N>(r, v, m, c);
@@ -246,22 +251,36 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         {
             if((batch & (batch - 1)) == 0)             // batches 0, 1, 2, 4, 8 ...
             {
-                const float mine = warp_reached_by(r.m, wanted);
+                const float mine = warp_reached_by(r.m, second, wanted);
                 if(lane == 0) shared.warp_top[warp] = mine;
                 // the first bound needs every warp's; later ones take what is there, since bounds only rise
                 if(batch == 0) __syncthreads();
+                else __syncwarp();
                 bound = shared.warp_top[0];
 #pragma unroll
                 for(int w = 1; w < kWarps; w++) bound = fminf(bound, shared.warp_top[w]);
+                bound = fmaxf(bound, -FLT_MAX);
             }
 #pragma unroll
             for(int u = 0; u < N; u++)
             {
-                if(vector_max[u] < bound || vector_max[u] == -INFINITY) continue;
-                const int at = atomicAdd(&shared.hits, 1);
-                if(at < kHits) { shared.hit[at] = v[u]; shared.hit_index[at] = cut.head + (first + u * kThreads + tid) * VE; }
+                const bool hit = vector_max[u] >= bound;
+                const unsigned int who = __ballot_sync(0xffffffffu, hit);
+                if(who == 0) continue;
+                const int at = hits + __popc(who & ((1u << lane) - 1u));
+                if(hit && at < kHits)
+                {
+                    shared.hit[warp][at] = v[u];
+                    shared.hit_index[warp][at] = cut.head + (first + u * kThreads + tid) * VE;
+                }
+                hits += __popc(who);
             }
         }
+    };
+    {
+        int first = begin, batch = 0;
+        for(; first + kThreads * N <= end; first += kThreads * N, batch++) take(first, batch, std::true_type{});
+        if(first < end || batch == 0) take(first, batch, std::false_type{});
     }
 
     // every warp's part to every CTA of the cluster
@@ -274,7 +293,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     part.w = warp_sum(r.w);
     const int parts = ctas * kWarps;
     const int wanted_all = TOP ? (top + parts - 1) / parts : 1;
-    part.top = TOP ? warp_reached_by(own_max, wanted_all) : 0.f;
+    part.top = TOP ? warp_reached_by(own_max, second, wanted_all) : 0.f;
     if(ctas == 1)
     {
         if(lane == 0) shared.parts[warp] = part;
@@ -335,29 +354,36 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             for(int i = lane; i < parts; i += 32) lowest = fminf(lowest, shared.parts[i].top);
             bound = -warp_max(-lowest);
         }
-        const int hits = shared.hits;
+        bound = fmaxf(bound, -FLT_MAX);                // -inf is no alternative
         Shared<TOP>* leader = ctas == 1 ? &shared : cluster.map_shared_rank(&shared, 0);
         auto candidate = [&](float value, int index)
         {
-            const unsigned long long key = key_of(value, index);
-            if(!(value >= bound) || key == 0) return;
+            if(!(value >= bound)) return;
             const int at = atomicAdd(&leader->candidate_count, 1);
-            if(at < kCandidates) leader->candidates[at] = key;
+            if(at < kCandidates) leader->candidates[at] = key_of(value, index);
         };
-        if(hits > kHits)
+        if(end_index >= 0) candidate(end_value, end_index);
+        if(hits <= kHits)
         {
-            if(tid == 0) atomicAdd(&leader->candidate_count, kCandidates + 1);
+            for(int i = lane; i < hits; i += 32)
+            {
+                float values[VE];
+                L::unpack(shared.hit[warp][i], values);
+                const int index = shared.hit_index[warp][i];
+#pragma unroll
+                for(int e = 0; e < VE; e++) candidate(values[e], index + e);
+            }
         }
         else
         {
-            if(end_index >= 0) candidate(end_value, end_index);
-            for(int i = tid; i < hits; i += kThreads)
+            for(int i = begin + tid; i < end; i += kThreads)
             {
+                const uint4 v = __ldg(body + i);
+                if(!(L::max(v) >= bound)) continue;
                 float values[VE];
-                L::unpack(shared.hit[i], values);
-                const int index = shared.hit_index[i];
+                L::unpack(v, values);
 #pragma unroll
-                for(int e = 0; e < VE; e++) candidate(values[e], index + e);
+                for(int e = 0; e < VE; e++) candidate(values[e], cut.head + i * VE + e);
             }
         }
         if(ctas == 1) __syncthreads();

@@ -186,6 +186,18 @@ def test_token_logprobs_many_ties_past_any_list(capi):
     check_logprobs(capi, x, None, 128, 1.0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_token_logprobs_runs_of_nan(capi, dtype):
+    """Stretches of NaN: the values are NaN, the ids those of the other logits in order."""
+    x = make_logits(4, 30000, dtype, seed=8)
+    x[0, 64:128] = math.nan
+    x[1, :29000] = math.nan
+    x[2] = math.nan
+    x[3, ::2] = math.nan
+    for top in (1, 3, 50, 128):
+        check_logprobs(capi, x, None, top, 1.0)
+
+
 def test_token_logprobs_each_output_alone(capi):
     x, tokens = make_logits(5, 999, "f32"), make_tokens(5, 999)
     full = capi.token_logprobs(x, tokens, top=7)
