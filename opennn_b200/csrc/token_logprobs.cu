@@ -18,8 +18,7 @@ namespace onn
 namespace
 {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 256;                     // of the backward pass
 constexpr int kUnroll = 8;                        // 16-byte vectors a thread has in flight
 
 // Running statistics of a set of logits, in base 2 and relative to the largest logit m seen: with c = log2(e) / T,
@@ -133,50 +132,55 @@ __device__ __forceinline__ float warp_reached_by(float first, float second, int 
 }
 
 constexpr int kMaxCluster = 8;
-constexpr int kHits = 160;                        // vectors with a possible alternative that a warp can hold
+constexpr int kMaxParts = 64;                     // warps that share a row: 8 CTAs of 8
+constexpr int kSlots = 16;                        // maxima a thread writes down
 constexpr int kCandidates = 1024;
+constexpr int kBuckets = 256;
 
 // What a warp knows of its part of the row.
 struct alignas(16) Part { float m, s, w, top; };
 
-// Shared memory of a CTA.  `parts` and, in the first CTA of a cluster, `candidates` are written by the whole cluster.
-template <bool TOP>
+// Shared memory of a CTA of T threads.  `parts` and, in the first CTA of a cluster, `candidates` are written by the whole
+// cluster.
+template <bool TOP, int T>
 struct Shared
 {
-    Part parts[kMaxCluster * kWarps];
+    Part parts[kMaxParts];
     float m, log_s;
 };
-template <>
-struct Shared<true>
+template <int T>
+struct Shared<true, T>
 {
-    Part parts[kMaxCluster * kWarps];
+    Part parts[kMaxParts];
     float m, log_s;
-    volatile float warp_top[kWarps];
-    int candidate_count;
-    unsigned long long best[kWarps];
-    uint4 hit[kWarps][kHits];
-    int hit_index[kWarps][kHits];
+    int candidate_count, kept_count, lowest_bucket;
+    unsigned long long best[T / 32];
     unsigned long long candidates[kCandidates];
+    union
+    {
+        float slot[kSlots][T];                    // the largest logit of each unit of vectors
+        struct { unsigned long long kept[kCandidates]; int bucket[kBuckets]; } thin;
+    };
+    unsigned short unit[T / 32][32 * kSlots];     // of each warp: units that hold an alternative
 };
 
 // One cluster of CTAs (often of one) per row; each CTA streams its part of the row once.
 //
-// The alternatives come out of the same pass.  If every warp knows k logits that are at least t, with k = ceil(top /
-// warps), no logit below t can stand in the list.  So after its first batch every warp takes the k-th largest of its
-// lanes' two best vectors as its bound; the smallest bound of all warps is the CTA's, and vectors with a logit that reaches
-// it go on the warp's list in shared memory (a compare per vector; for logits in no particular order a few hundred
-// of a row).  The bounds rise after 2, 3, 5, 9 ... batches.  At the end the bound of all warps thins the lists out to little
-// more than `top` candidates in the first CTA, which ranks them.  A list that overflows (a rising row) is replaced by
-// another scan with the final bound; candidates that overflow (a thousand equal logits) by a scan for each place.
-template <int DTYPE, bool TOP, int N>
-__global__ void __launch_bounds__(kThreads, N > 4 && TOP ? 3 : 4)
+// The alternatives: each thread also writes down the largest logit of each unit of its vectors (a vector, or some
+// batches of a long row).  If every warp knows k logits that are at least t, with k = ceil(top / warps), no logit below t can
+// stand in the list; so the k-th largest of the lanes' two best units is the warp's bound, and the smallest bound of all warps
+// the row's.  Only units that reach it (little more than `top` of them) are read again, most often from L2, and
+// their logits that reach it become candidates in the first CTA, which ranks them.  Should a thousand logits reach
+// the bound (equal ones), the row is scanned once for each place.
+template <int DTYPE, bool TOP, int T, int N>
+__global__ void __launch_bounds__(T, T == 32 ? 24 : 1024 / T)
 token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, long long pitch, const float* __restrict__ tokens,
                       float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ lse,
                       int* __restrict__ top_ids, float* __restrict__ top_logprobs, int top, int V, float c, float inverse_temperature)
 {
     using L = Logit<DTYPE>;
-    constexpr int VE = L::VE;
-    __shared__ Shared<TOP> shared;
+    constexpr int VE = L::VE, kWarps = T / 32;
+    __shared__ Shared<TOP, T> shared;
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const long long row = blockIdx.x / ctas;
@@ -193,7 +197,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             if(entropy) entropy[row] = 0.f;
             if(lse) lse[row] = 0.f;
         }
-        for(int k = tid; k < top; k += kThreads) { top_ids[row * top + k] = -1; top_logprobs[row * top + k] = -INFINITY; }
+        for(int k = tid; k < top; k += T) { top_ids[row * top + k] = -1; top_logprobs[row * top + k] = -INFINITY; }
         return;
     }
 
@@ -207,13 +211,21 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     const int share = (cut.vectors + ctas - 1) / ctas;
     const int begin = min(rank * share, cut.vectors), end = min(begin + share, cut.vectors);
 
+    // vectors of a unit: 1 << unit_shift; a thread has at most kSlots units
+    constexpr int kBatchShift = N == 8 ? 3 : 2;
+    const int each = (share + T - 1) / T;              // vectors of a thread
+    int unit_shift = 0;
+    if(TOP && each > kSlots)
+    {
+        unit_shift = kBatchShift;
+        while(((each - 1) >> unit_shift) >= kSlots) unit_shift++;
+    }
     if constexpr(TOP)
     {
-        if(tid == 0) shared.candidate_count = 0;
+        if(tid == 0) { shared.candidate_count = 0; shared.kept_count = 0; }
     }
     // all CTAs of a cluster must be running before one writes into another
     if(ctas > 1) cluster.sync();
-    else if constexpr(TOP) __syncthreads();
 
     Running r = {-INFINITY, 0.f, 0.f};
     float end_value = -INFINITY;
@@ -222,69 +234,64 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         end_value = L::get(x + end_index);
         // as a batch of its own; NaN is never larger, and reaches the sum
         r.m = end_value > -INFINITY ? end_value : -INFINITY;
-        r.s = exp2_approx(fmaf(end_value, c, -anchor(r.m, c)));
-        r.w = r.s * fmaxf(fmaf(end_value, c, -anchor(r.m, c)), kNothing);
+        const float d = fmaf(end_value, c, -anchor(r.m, c));
+        r.s = exp2_approx(d);
+        r.w = r.s * fmaxf(d, kNothing);
     }
-    const int wanted = TOP ? (top + kWarps - 1) / kWarps : 1;
-    [[maybe_unused]] float bound = -FLT_MAX, second = -INFINITY;     // of this lane's vectors, the second largest maximum
-    [[maybe_unused]] int hits = 0;                                   // on the warp's list
-    auto take = [&](const int first, const int batch, auto whole)
+    // of this thread's units
+    [[maybe_unused]] float best = -INFINITY, second = -INFINITY, unit_max = -INFINITY;
+    auto note = [&](float value, int slot)
     {
+        if constexpr(TOP)
+        {
+            shared.slot[slot][tid] = value;
+            second = fmaxf(second, value > best ? best : value);       // NaN is passed by
+            best = fmaxf(best, value);
+        }
+    };
+    auto take = [&](const int batch, auto whole)
+    {
+        const int first = begin + batch * (T * N);
         uint4 v[N];
 #pragma unroll
         for(int u = 0; u < N; u++)
         {
-            const int i = first + u * kThreads + tid;
+            const int i = first + u * T + tid;
             v[u] = whole.value || i < end ? __ldg(body + i) : L::lowest();
         }
         float vector_max[N];
-        float m = r.m;
+        float m = -INFINITY;
 #pragma unroll
         for(int u = 0; u < N; u++)
         {
             vector_max[u] = L::max(v[u]);
-            if constexpr(TOP) second = fmaxf(second, vector_max[u] > m ? m : vector_max[u]);       // NaN is passed by
             m = fmaxf(m, vector_max[u]);
         }
-        add_vectors<DTYPE, N>(r, v, m, c);
         if constexpr(TOP)
         {
-            if((batch & (batch - 1)) == 0)             // batches 0, 1, 2, 4, 8 ...
+            if(unit_shift == 0)
             {
-                const float mine = warp_reached_by(r.m, second, wanted);
-                if(lane == 0) shared.warp_top[warp] = mine;
-                // the first bound needs every warp's; later ones take what is there, since bounds only rise
-                if(batch == 0) __syncthreads();
-                else __syncwarp();
-                bound = shared.warp_top[0];
 #pragma unroll
-                for(int w = 1; w < kWarps; w++) bound = fminf(bound, shared.warp_top[w]);
-                bound = fmaxf(bound, -FLT_MAX);
+                for(int u = 0; u < N; u++)
+                    if(batch * N + u < each) note(vector_max[u], batch * N + u);
             }
-#pragma unroll
-            for(int u = 0; u < N; u++)
+            else
             {
-                const bool hit = vector_max[u] >= bound;
-                const unsigned int who = __ballot_sync(0xffffffffu, hit);
-                if(who == 0) continue;
-                const int at = hits + __popc(who & ((1u << lane) - 1u));
-                if(hit && at < kHits)
-                {
-                    shared.hit[warp][at] = v[u];
-                    shared.hit_index[warp][at] = cut.head + (first + u * kThreads + tid) * VE;
-                }
-                hits += __popc(who);
+                unit_max = fmaxf(unit_max, m);
+                const int last = ((batch + 1) * N - 1) >> unit_shift;
+                if(((batch + 1) * N) >> unit_shift != last || (batch + 1) * N >= each) { note(unit_max, last); unit_max = -INFINITY; }
             }
         }
+        add_vectors<DTYPE, N>(r, v, fmaxf(r.m, m), c);
     };
     {
-        int first = begin, batch = 0;
-        for(; first + kThreads * N <= end; first += kThreads * N, batch++) take(first, batch, std::true_type{});
-        if(first < end || batch == 0) take(first, batch, std::false_type{});
+        const int whole = (end - begin) / (T * N), batches = (each + N - 1) / N;
+        int batch = 0;
+        for(; batch < whole; batch++) take(batch, std::true_type{});
+        for(; batch < batches; batch++) take(batch, std::false_type{});
     }
 
     // every warp's part to every CTA of the cluster
-    const float own_max = r.m;
     const float warp_m = warp_max(r.m);
     rebase(r, warp_m, c);
     Part part;
@@ -292,8 +299,8 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     part.s = warp_sum(r.s);
     part.w = warp_sum(r.w);
     const int parts = ctas * kWarps;
-    const int wanted_all = TOP ? (top + parts - 1) / parts : 1;
-    part.top = TOP ? warp_reached_by(own_max, second, wanted_all) : 0.f;
+    const int wanted = TOP ? (top + parts - 1) / parts : 1;
+    part.top = TOP ? warp_reached_by(best, second, wanted) : 0.f;
     if(ctas == 1)
     {
         if(lane == 0) shared.parts[warp] = part;
@@ -309,9 +316,13 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     {
         Running all = {-INFINITY, 0.f, 0.f};
         for(int i = lane; i < parts; i += 32) all = merge(all, Running{shared.parts[i].m, shared.parts[i].s, shared.parts[i].w}, c);
-        rebase(all, warp_max(all.m), c);
-        all.s = warp_sum(all.s);
-        all.w = warp_sum(all.w);
+        if(parts > 1)
+        {
+            rebase(all, warp_max(all.m), c);
+            all.s = warp_sum(all.s);
+            all.w = warp_sum(all.w);
+        }
+        else all = Running{part.m, part.s, part.w};
         const bool huge = fabsf(all.m) >= kHuge && fabsf(all.m) < INFINITY;
         if(huge) all = huge_row<DTYPE>(x, V, all.m, c);
         if(lane == 0)
@@ -334,8 +345,8 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
 
     if constexpr(TOP)
     {
-        // the bound of all maxima
-        if(wanted_all == 1 && parts >= 2 * top)
+        float bound;
+        if(wanted == 1 && parts >= 2 * top)
         {
             // more warps than places: the bound is the top-th largest of their maxima
             float found = -INFINITY;
@@ -355,35 +366,62 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             bound = -warp_max(-lowest);
         }
         bound = fmaxf(bound, -FLT_MAX);                // -inf is no alternative
-        Shared<TOP>* leader = ctas == 1 ? &shared : cluster.map_shared_rank(&shared, 0);
+
+        Shared<TOP, T>* leader = ctas == 1 ? &shared : cluster.map_shared_rank(&shared, 0);
         auto candidate = [&](float value, int index)
         {
-            if(!(value >= bound)) return;
             const int at = atomicAdd(&leader->candidate_count, 1);
             if(at < kCandidates) leader->candidates[at] = key_of(value, index);
         };
-        if(end_index >= 0) candidate(end_value, end_index);
-        if(hits <= kHits)
+        if(end_value >= bound) candidate(end_value, end_index);
+        // this warp's units that reach the bound, then their vectors, four loads of a lane at a time
+        unsigned short* units = shared.unit[warp];
+        int found = 0;
+        const int slots = each > 0 ? ((each - 1) >> unit_shift) + 1 : 0;
+        for(int slot = 0; slot < slots; slot++)
         {
-            for(int i = lane; i < hits; i += 32)
-            {
-                float values[VE];
-                L::unpack(shared.hit[warp][i], values);
-                const int index = shared.hit_index[warp][i];
-#pragma unroll
-                for(int e = 0; e < VE; e++) candidate(values[e], index + e);
-            }
+            const bool hit = shared.slot[slot][tid] >= bound;
+            const unsigned int who = __ballot_sync(0xffffffffu, hit);
+            if(hit) units[found + __popc(who & ((1u << lane) - 1u))] = (unsigned short)(slot * 32 + lane);
+            found += __popc(who);
         }
-        else
+        __syncwarp();
+        const int again = found << unit_shift;
+        for(int start = lane; start < again; start += 4 * 32)
         {
-            for(int i = begin + tid; i < end; i += kThreads)
-            {
-                const uint4 v = __ldg(body + i);
-                if(!(L::max(v) >= bound)) continue;
-                float values[VE];
-                L::unpack(v, values);
+            uint4 v[4];
+            int at[4];
 #pragma unroll
-                for(int e = 0; e < VE; e++) candidate(values[e], cut.head + i * VE + e);
+            for(int k = 0; k < 4; k++)
+            {
+                const int j = start + k * 32;
+                at[k] = end;
+                if(j < again)
+                {
+                    const int unit = units[j >> unit_shift];
+                    const int ordinal = ((unit >> 5) << unit_shift) + (j & ((1 << unit_shift) - 1));
+                    at[k] = begin + ordinal * T + warp * 32 + (unit & 31);
+                }
+                v[k] = at[k] < end ? __ldg(body + at[k]) : L::lowest();
+            }
+#pragma unroll
+            for(int k = 0; k < 4; k++)
+            {
+                if(!(L::max(v[k]) >= bound)) continue;
+                float values[VE];
+                L::unpack(v[k], values);
+                unsigned int which = 0;
+#pragma unroll
+                for(int e = 0; e < VE; e++) which |= (values[e] >= bound ? 1u : 0u) << e;
+                while(which)
+                {
+                    const int e = __ffs(which) - 1;
+                    which &= which - 1;
+                    float value = values[0];
+#pragma unroll
+                    for(int i = 1; i < VE; i++) value = e == i ? values[i] : value;
+                    candidate(value, cut.head + at[k] * VE + e);
+                }
             }
         }
         if(ctas == 1) __syncthreads();
@@ -402,16 +440,16 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             unsigned long long last = ~0ull;
             for(int k = 0; k < top; k++)
             {
-                unsigned long long best = 0;
+                unsigned long long largest = 0;
                 auto look = [&](float value, int index)
                 {
                     const unsigned long long key = key_of(value, index);
-                    if(key < last && key > best) best = key;
+                    if(key < last && key > largest) largest = key;
                 };
                 if(last != 0)
                 {
                     if(end_index >= 0) look(end_value, end_index);
-                    for(int i = tid; i < cut.vectors; i += kThreads)
+                    for(int i = tid; i < cut.vectors; i += T)
                     {
                         float values[VE];
                         L::unpack(__ldg(body + i), values);
@@ -422,52 +460,90 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
 #pragma unroll
                 for(int offset = 16; offset > 0; offset >>= 1)
                 {
-                    const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, offset);
-                    best = other > best ? other : best;
+                    const unsigned long long other = __shfl_xor_sync(0xffffffffu, largest, offset);
+                    largest = other > largest ? other : largest;
                 }
                 __syncthreads();
-                if(lane == 0) shared.best[warp] = best;
+                if(lane == 0) shared.best[warp] = largest;
                 __syncthreads();
-                best = shared.best[0];
+                largest = shared.best[0];
 #pragma unroll
-                for(int w = 1; w < kWarps; w++) best = shared.best[w] > best ? shared.best[w] : best;
-                last = best;
-                if(tid == 0) place(k, best);
+                for(int w = 1; w < kWarps; w++) largest = shared.best[w] > largest ? shared.best[w] : largest;
+                last = largest;
+                if(tid == 0) place(k, largest);
             }
             return;
         }
-        for(int k = n + tid; k < top; k += kThreads) place(k, 0);
-        if(n <= kThreads)
+        for(int k = n + tid; k < top; k += T) place(k, 0);
+
+        const unsigned long long* keys = shared.candidates;
+        if(n > top + 128)
         {
-            // few: a candidate's place is the number of larger ones
-            if(tid < n)
+            // many more than places: evenly spaced buckets between the lowest and the largest candidate, of which only those from
+            // the one that holds the last place upwards are kept
+            unsigned long long lowest_key = ~0ull, largest_key = 0;
+            for(int i = tid; i < n; i += T)
             {
-                const unsigned long long key = shared.candidates[tid];
-                int larger = 0;
-#pragma unroll 4
-                for(int j = 0; j < n; j++) larger += shared.candidates[j] > key;
-                if(larger < top) place(larger, key);
+                lowest_key = min(lowest_key, shared.candidates[i]);
+                largest_key = max(largest_key, shared.candidates[i]);
             }
-            return;
-        }
-        int padded = 2 * kThreads;
-        while(padded < n) padded *= 2;
-        for(int i = n + tid; i < padded; i += kThreads) shared.candidates[i] = 0;
-        for(int size = 2; size <= padded; size <<= 1)
-        {
-            for(int stride = size >> 1; stride > 0; stride >>= 1)
+#pragma unroll
+            for(int offset = 16; offset > 0; offset >>= 1)
             {
-                __syncthreads();
-                for(int pair = tid; pair < padded / 2; pair += kThreads)
+                lowest_key = min(lowest_key, __shfl_xor_sync(0xffffffffu, lowest_key, offset));
+                largest_key = max(largest_key, __shfl_xor_sync(0xffffffffu, largest_key, offset));
+            }
+            for(int i = tid; i < kBuckets; i += T) shared.thin.bucket[i] = 0;      // the slots have been read by all
+            if(lane == 0) shared.parts[warp] = Part{key_logit(lowest_key), key_logit(largest_key), 0.f, 0.f};
+            __syncthreads();
+            float low = shared.parts[0].m, high = shared.parts[0].s;
+            for(int w = 1; w < kWarps; w++) { low = fminf(low, shared.parts[w].m); high = fmaxf(high, shared.parts[w].s); }
+            // a warp without candidates has said NaN, which the minimum and the maximum pass by; halves, so that the width is finite
+            const float width = high * 0.5f - low * 0.5f;
+            const float per = width > 0.f && width < INFINITY ? 0.5f * (kBuckets - 1) / width : 0.f;
+            auto bucket_of = [&](unsigned long long key) { return min(kBuckets - 1, (int)((key_logit(key) * 0.5f - low * 0.5f) * (2.f * per))); };
+            for(int i = tid; i < n; i += T) atomicAdd(&shared.thin.bucket[bucket_of(shared.candidates[i])], 1);
+            __syncthreads();
+            if(warp == 0)
+            {
+                // lane l has the buckets from the top: 255 - 8 l downwards
+                int mine = 0;
+                for(int b = 0; b < kBuckets / 32; b++) mine += shared.thin.bucket[kBuckets - 1 - lane * (kBuckets / 32) - b];
+                int above = mine;
+#pragma unroll
+                for(int offset = 1; offset < 32; offset <<= 1)
                 {
-                    const int i = 2 * pair - (pair & (stride - 1)), j = i + stride;
-                    const unsigned long long a = shared.candidates[i], b = shared.candidates[j];
-                    if(((i & size) == 0) != (a > b)) { shared.candidates[i] = b; shared.candidates[j] = a; }
+                    const int other = __shfl_up_sync(0xffffffffu, above, offset);
+                    if(lane >= offset) above += other;
+                }
+                above -= mine;
+                if(above < top && above + mine >= top)
+                {
+                    int b = kBuckets - 1 - lane * (kBuckets / 32);
+                    while((above += shared.thin.bucket[b]) < top) b--;
+                    shared.lowest_bucket = b;
                 }
             }
+            __syncthreads();
+            const int lowest_bucket = shared.lowest_bucket;
+            for(int i = tid; i < n; i += T)
+            {
+                const unsigned long long key = shared.candidates[i];
+                if(bucket_of(key) >= lowest_bucket) shared.thin.kept[atomicAdd(&shared.kept_count, 1)] = key;
+            }
+            __syncthreads();
+            keys = shared.thin.kept;
+            n = shared.kept_count;
         }
-        __syncthreads();
-        for(int k = tid; k < min(top, n); k += kThreads) place(k, shared.candidates[k]);
+        // a candidate's place is the number of larger ones
+        for(int i = tid; i < n; i += T)
+        {
+            const unsigned long long key = keys[i];
+            int larger = 0;
+#pragma unroll 4
+            for(int j = 0; j < n; j++) larger += keys[j] > key;
+            if(larger < top) place(larger, key);
+        }
     }
 }
 
@@ -534,16 +610,14 @@ token_logprobs_bwd_kernel(const typename Logit<DTYPE>::type* logits, long long p
     }
 }
 
-template <int DTYPE, bool TOP, int N>
+template <int DTYPE, bool TOP, int T>
 int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float* logprobs, float* entropy, float* lse,
                   int32_t* top_ids, float* top_logprobs, int64_t top, int64_t rows, int64_t V, float c, float inverse_temperature,
-                  cudaStream_t stream)
+                  int ctas, cudaStream_t stream)
 {
     using L = Logit<DTYPE>;
-    // few rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read
-    int ctas = 1;
-    while(ctas < kMaxCluster && rows * ctas * 2 <= 4 * kSmCount && V / L::VE >= (int64_t)ctas * 2 * kThreads * 2) ctas *= 2;
-    if(launch_clusters(token_logprobs_kernel<DTYPE, TOP, N>, (unsigned)(rows * ctas), kThreads, ctas, stream,
+    constexpr int N = DTYPE == ONN_F32 ? 8 : 4;
+    if(launch_clusters(token_logprobs_kernel<DTYPE, TOP, T, N>, (unsigned)(rows * ctas), T, ctas, stream,
                        static_cast<const typename L::type*>(logits), (long long)pitch, tokens, logprobs, entropy, lse, top_ids,
                        top_logprobs, (int)top, (int)V, c, inverse_temperature) != cudaSuccess) return ONN_ERR_CUDA;
     count_launch();
@@ -555,9 +629,15 @@ int launch_fwd(const void* logits, int64_t pitch, const float* tokens, float* lo
                int32_t* top_ids, float* top_logprobs, int64_t top, int64_t rows, int64_t V, float c, float inverse_temperature,
                cudaStream_t stream)
 {
-    constexpr int N = DTYPE == ONN_F32 ? 8 : 4;
-    const auto launch = top > 0 ? launch_fwd_as<DTYPE, true, N> : launch_fwd_as<DTYPE, false, N>;
-    return launch(logits, pitch, tokens, logprobs, entropy, lse, top_ids, top_logprobs, top, rows, V, c, inverse_temperature, stream);
+    const int64_t vectors = V / Logit<DTYPE>::VE;
+    static const int forced = []{ const char* e = getenv("X_T"); return e ? atoi(e) : 0; }();
+    int T = forced ? forced : 256;
+    // few rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read
+    int ctas = 1;
+    while(T == 256 && ctas < kMaxCluster && rows * ctas * 2 <= 4 * kSmCount && vectors >= (int64_t)ctas * 2 * T * 2) ctas *= 2;
+    const auto launch = top > 0 ? (T == 32 ? launch_fwd_as<DTYPE, true, 32> : T == 128 ? launch_fwd_as<DTYPE, true, 128> : launch_fwd_as<DTYPE, true, 256>)
+                                : (T == 32 ? launch_fwd_as<DTYPE, false, 32> : T == 128 ? launch_fwd_as<DTYPE, false, 128> : launch_fwd_as<DTYPE, false, 256>);
+    return launch(logits, pitch, tokens, logprobs, entropy, lse, top_ids, top_logprobs, top, rows, V, c, inverse_temperature, ctas, stream);
 }
 
 template <int DTYPE>
