@@ -136,6 +136,7 @@ constexpr int kMaxParts = 64;                     // warps that share a row: 8 C
 constexpr int kSlots = 16;                        // maxima a thread writes down
 constexpr int kCandidates = 1024;
 constexpr int kBuckets = 256;
+constexpr int kFew = 96;                          // candidates that are ranked without buckets
 
 // What a warp knows of its part of the row.
 struct alignas(16) Part { float m, s, w, top; };
@@ -145,26 +146,26 @@ struct alignas(16) Part { float m, s, w, top; };
 template <bool TOP, int T>
 struct Shared
 {
-    Part parts[kMaxParts];
-    float m, log_s;
+    Part parts[2][kMaxParts];                     // of this row and the next
 };
 template <int T>
 struct Shared<true, T>
 {
-    Part parts[kMaxParts];
+    Part parts[2][kMaxParts];
     float m, log_s;
-    int candidate_count, kept_count, lowest_bucket;
+    int candidate_count;
+    int bucket[kBuckets + 1];
     unsigned long long best[T / 32];
     unsigned long long candidates[kCandidates];
     union
     {
         float slot[kSlots][T];                    // the largest logit of each unit of vectors
-        struct { unsigned long long kept[kCandidates]; int bucket[kBuckets]; } thin;
+        unsigned long long sorted[kCandidates];
     };
     unsigned short unit[T / 32][32 * kSlots];     // of each warp: units that hold an alternative
 };
 
-// One cluster of CTAs (often of one) per row; each CTA streams its part of the row once.
+// Clusters of CTAs (often of one) walk over the rows; each CTA streams its part of a row once.
 //
 // The alternatives: each thread also writes down the largest logit of each unit of its vectors (a vector, or some
 // batches of a long row).  If every warp knows k logits that are at least t, with k = ceil(top / warps), no logit below t can
@@ -176,30 +177,47 @@ template <int DTYPE, bool TOP, int T, int N>
 __global__ void __launch_bounds__(T, T == 32 ? 24 : 1024 / T)
 token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, long long pitch, const float* __restrict__ tokens,
                       float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ lse,
-                      int* __restrict__ top_ids, float* __restrict__ top_logprobs, int top, int V, float c, float inverse_temperature)
+                      int* __restrict__ top_ids, float* __restrict__ top_logprobs, int top, long long rows, int V, float c, float inverse_temperature)
 {
     using L = Logit<DTYPE>;
     constexpr int VE = L::VE, kWarps = T / 32;
     __shared__ Shared<TOP, T> shared;
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const long long row = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if constexpr(TOP)
+    {
+        if(tid == 0) shared.candidate_count = 0;
+        for(int i = tid; i <= kBuckets; i += T) shared.bucket[i] = 0;
+    }
+    // all CTAs of a cluster must be running before one writes into another
+    if(ctas > 1) cluster.sync();
 
-    bool active;
-    const long long token = row_token(tokens, row, V, &active);
+    int flip = 0;
+    const long long step = gridDim.x / ctas;
+    long long row = blockIdx.x / ctas;
+    float next_token = tokens && row < rows ? __ldg(tokens + row) : 1.f;
+    for(; row < rows; row += step)
+    {
+    const long long token = token_index(next_token);
+    const bool active = token > 0 && token < V;        // 0 is padding; without tokens every row takes part
+    if(tokens && row + step < rows) next_token = __ldg(tokens + row + step);
     if(!active)                                        // the same for the whole cluster
     {
-        if(rank != 0) return;
-        if(tid == 0)
+        if(rank == 0)
         {
-            if(logprobs) logprobs[row] = 0.f;
-            if(entropy) entropy[row] = 0.f;
-            if(lse) lse[row] = 0.f;
+            if(tid == 0)
+            {
+                if(logprobs) logprobs[row] = 0.f;
+                if(entropy) entropy[row] = 0.f;
+                if(lse) lse[row] = 0.f;
+            }
+            for(int k = tid; k < top; k += T) { top_ids[row * top + k] = -1; top_logprobs[row * top + k] = -INFINITY; }
         }
-        for(int k = tid; k < top; k += T) { top_ids[row * top + k] = -1; top_logprobs[row * top + k] = -INFINITY; }
-        return;
+        continue;
     }
+    flip ^= 1;
+    Part* const row_parts = shared.parts[flip];
 
     const typename L::type* x = logits + row * pitch;
     const RowCut cut = cut_row<DTYPE>(x, V);
@@ -220,13 +238,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         unit_shift = kBatchShift;
         while(((each - 1) >> unit_shift) >= kSlots) unit_shift++;
     }
-    if constexpr(TOP)
-    {
-        if(tid == 0) { shared.candidate_count = 0; shared.kept_count = 0; }
-    }
-    // all CTAs of a cluster must be running before one writes into another
-    if(ctas > 1) cluster.sync();
-
+    const float given = tid == 0 && rank == 0 ? L::get(x + token) : 0.f;
     Running r = {-INFINITY, 0.f, 0.f};
     float end_value = -INFINITY;
     if(end_index >= 0)
@@ -303,19 +315,19 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     part.top = TOP ? warp_reached_by(best, second, wanted) : 0.f;
     if(ctas == 1)
     {
-        if(lane == 0) shared.parts[warp] = part;
+        if(lane == 0) row_parts[warp] = part;
         __syncthreads();
     }
     else
     {
-        if(lane < ctas) cluster.map_shared_rank(&shared, lane)->parts[rank * kWarps + warp] = part;
+        if(lane < ctas) cluster.map_shared_rank(&shared, lane)->parts[flip][rank * kWarps + warp] = part;
         cluster.sync();
     }
 
     if(rank == 0 && warp == 0)
     {
         Running all = {-INFINITY, 0.f, 0.f};
-        for(int i = lane; i < parts; i += 32) all = merge(all, Running{shared.parts[i].m, shared.parts[i].s, shared.parts[i].w}, c);
+        for(int i = lane; i < parts; i += 32) all = merge(all, Running{row_parts[i].m, row_parts[i].s, row_parts[i].w}, c);
         if(parts > 1)
         {
             rebase(all, warp_max(all.m), c);
@@ -331,9 +343,8 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             const float log_2s = logf(all.s);
             // relative to m itself: the rounding of the anchor
             const float log_s = none ? INFINITY : huge ? log_2s : fmaf(fmaf(all.m, c, -anchor(all.m, c)), -kLn2, log_2s);
-            shared.m = finite_anchor(all.m);
-            shared.log_s = log_s;
-            if(logprobs) logprobs[row] = none ? -INFINITY : (L::get(x + token) - all.m) * inverse_temperature - log_s;
+            if constexpr(TOP) { shared.m = finite_anchor(all.m); shared.log_s = log_s; }
+            if(logprobs) logprobs[row] = none ? -INFINITY : (given - all.m) * inverse_temperature - log_s;
             if(entropy)
             {
                 const float value = log_2s - all.w / all.s * kLn2;
@@ -352,9 +363,9 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             float found = -INFINITY;
             for(int i = lane; i < parts; i += 32)
             {
-                const float mine = shared.parts[i].m;
+                const float mine = row_parts[i].m;
                 int larger = 0;
-                for(int j = 0; j < parts; j++) larger += shared.parts[j].m > mine || (shared.parts[j].m == mine && j < i);
+                for(int j = 0; j < parts; j++) larger += row_parts[j].m > mine || (row_parts[j].m == mine && j < i);
                 if(larger == top - 1) found = mine;
             }
             bound = warp_max(found);
@@ -362,7 +373,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         else
         {
             float lowest = INFINITY;
-            for(int i = lane; i < parts; i += 32) lowest = fminf(lowest, shared.parts[i].top);
+            for(int i = lane; i < parts; i += 32) lowest = fminf(lowest, row_parts[i].top);
             bound = -warp_max(-lowest);
         }
         bound = fmaxf(bound, -FLT_MAX);                // -inf is no alternative
@@ -426,15 +437,14 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         }
         if(ctas == 1) __syncthreads();
         else cluster.sync();
-        if(rank != 0) return;
-
         auto place = [&](int k, unsigned long long key)
         {
             top_ids[row * top + k] = key ? key_index(key) : -1;
             top_logprobs[row * top + k] = key ? (key_logit(key) - shared.m) * inverse_temperature - shared.log_s : -INFINITY;
         };
-        int n = shared.candidate_count;
-        if(n > kCandidates)
+        int n = rank == 0 ? shared.candidate_count : 0;
+        if(rank != 0) {}
+        else if(n > kCandidates)
         {
             // one place after the other: the largest key below the last one
             unsigned long long last = ~0ull;
@@ -472,79 +482,90 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
                 last = largest;
                 if(tid == 0) place(k, largest);
             }
-            return;
         }
+        else
+        {
         for(int k = n + tid; k < top; k += T) place(k, 0);
 
-        const unsigned long long* keys = shared.candidates;
-        if(n > top + 128)
+        // A candidate's place is the number of larger ones: those of higher buckets, of kBuckets that lie evenly between the
+        // bound and the largest logit, and those before it in its own.  bucket[b + 1] counts bucket b, 0 is the highest.
+        if(n <= kFew)
         {
-            // many more than places: evenly spaced buckets between the lowest and the largest candidate, of which only those from
-            // the one that holds the last place upwards are kept
-            unsigned long long lowest_key = ~0ull, largest_key = 0;
-            for(int i = tid; i < n; i += T)
-            {
-                lowest_key = min(lowest_key, shared.candidates[i]);
-                largest_key = max(largest_key, shared.candidates[i]);
-            }
-#pragma unroll
-            for(int offset = 16; offset > 0; offset >>= 1)
-            {
-                lowest_key = min(lowest_key, __shfl_xor_sync(0xffffffffu, lowest_key, offset));
-                largest_key = max(largest_key, __shfl_xor_sync(0xffffffffu, largest_key, offset));
-            }
-            for(int i = tid; i < kBuckets; i += T) shared.thin.bucket[i] = 0;      // the slots have been read by all
-            if(lane == 0) shared.parts[warp] = Part{key_logit(lowest_key), key_logit(largest_key), 0.f, 0.f};
-            __syncthreads();
-            float low = shared.parts[0].m, high = shared.parts[0].s;
-            for(int w = 1; w < kWarps; w++) { low = fminf(low, shared.parts[w].m); high = fmaxf(high, shared.parts[w].s); }
-            // a warp without candidates has said NaN, which the minimum and the maximum pass by; halves, so that the width is finite
-            const float width = high * 0.5f - low * 0.5f;
-            const float per = width > 0.f && width < INFINITY ? 0.5f * (kBuckets - 1) / width : 0.f;
-            auto bucket_of = [&](unsigned long long key) { return min(kBuckets - 1, (int)((key_logit(key) * 0.5f - low * 0.5f) * (2.f * per))); };
-            for(int i = tid; i < n; i += T) atomicAdd(&shared.thin.bucket[bucket_of(shared.candidates[i])], 1);
-            __syncthreads();
-            if(warp == 0)
-            {
-                // lane l has the buckets from the top: 255 - 8 l downwards
-                int mine = 0;
-                for(int b = 0; b < kBuckets / 32; b++) mine += shared.thin.bucket[kBuckets - 1 - lane * (kBuckets / 32) - b];
-                int above = mine;
-#pragma unroll
-                for(int offset = 1; offset < 32; offset <<= 1)
-                {
-                    const int other = __shfl_up_sync(0xffffffffu, above, offset);
-                    if(lane >= offset) above += other;
-                }
-                above -= mine;
-                if(above < top && above + mine >= top)
-                {
-                    int b = kBuckets - 1 - lane * (kBuckets / 32);
-                    while((above += shared.thin.bucket[b]) < top) b--;
-                    shared.lowest_bucket = b;
-                }
-            }
-            __syncthreads();
-            const int lowest_bucket = shared.lowest_bucket;
             for(int i = tid; i < n; i += T)
             {
                 const unsigned long long key = shared.candidates[i];
-                if(bucket_of(key) >= lowest_bucket) shared.thin.kept[atomicAdd(&shared.kept_count, 1)] = key;
+                int larger = 0;
+#pragma unroll 4
+                for(int j = 0; j < n; j++) larger += shared.candidates[j] > key;
+                if(larger < top) place(larger, key);
             }
-            __syncthreads();
-            keys = shared.thin.kept;
-            n = shared.kept_count;
         }
-        // a candidate's place is the number of larger ones
+        else
+        {
+        const float high = shared.m;
+        float low = bound;
+        if(bound == -FLT_MAX)
+        {
+            // no bound: the lowest candidate
+            float lowest = INFINITY;
+            for(int i = tid; i < n; i += T) lowest = fminf(lowest, key_logit(shared.candidates[i]));
+            lowest = -warp_max(-lowest);
+            if(lane == 0) row_parts[warp].m = lowest;
+            __syncthreads();
+            low = row_parts[0].m;
+#pragma unroll
+            for(int w = 1; w < kWarps; w++) low = fminf(low, row_parts[w].m);
+        }
+        const float width = high * 0.5f - low * 0.5f;   // halves: finite whatever the two are
+        const float per = width > 0.f && width < INFINITY ? (kBuckets - 1) / width : 0.f;
+        auto bucket_of = [&](unsigned long long key) { return min(kBuckets - 1, (int)((high * 0.5f - key_logit(key) * 0.5f) * per)); };
+        for(int i = tid; i < n; i += T) atomicAdd(&shared.bucket[bucket_of(shared.candidates[i]) + 1], 1);
+        __syncthreads();
+        if(warp == 0)
+        {
+            // running sums: bucket[b + 1] becomes the number of candidates in the buckets up to b
+            int mine[kBuckets / 32], total = 0;
+#pragma unroll
+            for(int b = 0; b < kBuckets / 32; b++) { mine[b] = shared.bucket[lane * (kBuckets / 32) + b + 1]; total += mine[b]; }
+            int before = total;
+#pragma unroll
+            for(int offset = 1; offset < 32; offset <<= 1)
+            {
+                const int other = __shfl_up_sync(0xffffffffu, before, offset);
+                if(lane >= offset) before += other;
+            }
+            before -= total;
+#pragma unroll
+            for(int b = 0; b < kBuckets / 32; b++) { shared.bucket[lane * (kBuckets / 32) + b + 1] = before; before += mine[b]; }
+        }
+        __syncthreads();
+        // bucket[b + 1] goes from where bucket b starts to where it ends, which is where the next one starts
         for(int i = tid; i < n; i += T)
         {
-            const unsigned long long key = keys[i];
-            int larger = 0;
-#pragma unroll 4
-            for(int j = 0; j < n; j++) larger += keys[j] > key;
+            const unsigned long long key = shared.candidates[i];
+            shared.sorted[atomicAdd(&shared.bucket[bucket_of(key) + 1], 1)] = key;
+        }
+        __syncthreads();
+        for(int i = tid; i < n; i += T)
+        {
+            const unsigned long long key = shared.sorted[i];
+            const int b = bucket_of(key), first = shared.bucket[b], end_of = shared.bucket[b + 1];
+            if(first >= top) continue;
+            int larger = first;
+            for(int j = first; j < end_of; j++) larger += shared.sorted[j] > key;
             if(larger < top) place(larger, key);
         }
+        __syncthreads();
+        for(int i = tid; i <= kBuckets; i += T) shared.bucket[i] = 0;
+        }
+        }
+        // the lists have been read before the next row's are written
+        __syncthreads();
+        if(tid == 0) shared.candidate_count = 0;
     }
+    }
+    // no CTA of a cluster ends while another may still write into it
+    if(ctas > 1) cluster.sync();
 }
 
 // One CTA per piece of a row: the row's scalars, then load, compute, store.
@@ -616,25 +637,33 @@ int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float*
                   int ctas, cudaStream_t stream)
 {
     using L = Logit<DTYPE>;
-    constexpr int N = DTYPE == ONN_F32 ? 8 : 4;
-    if(launch_clusters(token_logprobs_kernel<DTYPE, TOP, T, N>, (unsigned)(rows * ctas), T, ctas, stream,
+    // eight vectors in flight per thread; in 16 bits with a list four: the row's units are finer, and 8 CTAs of 128 threads fit
+    constexpr int N = DTYPE != ONN_F32 && TOP ? 4 : 8;
+    // single warps walk over the rows (27 us against 35 for 16384 rows of 1000 logits); larger CTAs have one row each, so that
+    // whoever is free takes the next (203 us against 213 for 8192 rows of 50021 with 64 alternatives)
+    int64_t clusters = rows;
+    if(T == 32 && clusters > 24 * kSmCount) clusters = 24 * kSmCount;
+    if(launch_clusters(token_logprobs_kernel<DTYPE, TOP, T, N>, (unsigned)(clusters * ctas), T, ctas, stream,
                        static_cast<const typename L::type*>(logits), (long long)pitch, tokens, logprobs, entropy, lse, top_ids,
-                       top_logprobs, (int)top, (int)V, c, inverse_temperature) != cudaSuccess) return ONN_ERR_CUDA;
+                       top_logprobs, (int)top, (long long)rows, (int)V, c, inverse_temperature) != cudaSuccess) return ONN_ERR_CUDA;
     count_launch();
     return launch_status();
 }
 
+// Threads of a row.  What a row costs besides its logits (start, reductions, ranking) is latency, so short rows want many
+// small CTAs: one warp up to 512 vectors (16384 x 1000 fp32: 27 us against 47 with 128 threads, 91 with 256), as
+// long as its 64 samples give a bound for the list (top <= 32).  A list of a long row wants more samples: 256 threads from
+// 12288 vectors (2048 x 131072 fp32 with 64 alternatives: 187 us against 212), else 128 (8192 x 50021 bf16: 203 against
+// 232).  Few rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read.
 template <int DTYPE>
 int launch_fwd(const void* logits, int64_t pitch, const float* tokens, float* logprobs, float* entropy, float* lse,
                int32_t* top_ids, float* top_logprobs, int64_t top, int64_t rows, int64_t V, float c, float inverse_temperature,
                cudaStream_t stream)
 {
     const int64_t vectors = V / Logit<DTYPE>::VE;
-    static const int forced = []{ const char* e = getenv("X_T"); return e ? atoi(e) : 0; }();
-    int T = forced ? forced : 256;
-    // few rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read
     int ctas = 1;
-    while(T == 256 && ctas < kMaxCluster && rows * ctas * 2 <= 4 * kSmCount && vectors >= (int64_t)ctas * 2 * T * 2) ctas *= 2;
+    while(ctas < kMaxCluster && rows * ctas * 2 <= 4 * kSmCount && vectors >= (int64_t)ctas * 1024) ctas *= 2;
+    const int T = ctas > 1 || (top > 0 && vectors >= 12288) ? 256 : vectors <= 512 && top <= 32 ? 32 : 128;
     const auto launch = top > 0 ? (T == 32 ? launch_fwd_as<DTYPE, true, 32> : T == 128 ? launch_fwd_as<DTYPE, true, 128> : launch_fwd_as<DTYPE, true, 256>)
                                 : (T == 32 ? launch_fwd_as<DTYPE, false, 32> : T == 128 ? launch_fwd_as<DTYPE, false, 128> : launch_fwd_as<DTYPE, false, 256>);
     return launch(logits, pitch, tokens, logprobs, entropy, lse, top_ids, top_logprobs, top, rows, V, c, inverse_temperature, ctas, stream);
