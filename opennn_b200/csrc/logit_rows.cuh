@@ -188,21 +188,23 @@ __device__ __forceinline__ long long row_token(const float* tokens, long long ro
     return t;
 }
 
-// A launch in clusters of `ctas` CTAs.
+// A launch in clusters of `ctas` CTAs.  overlapped: as launch_overlapped (the kernel calls pdl_wait first).
 template <typename... KernelArgs, typename... Args>
-inline cudaError_t launch_clusters(void (*kernel)(KernelArgs...), unsigned int grid, int threads, int ctas, cudaStream_t stream, Args&&... args)
+inline cudaError_t launch_clusters(void (*kernel)(KernelArgs...), unsigned int grid, int threads, int ctas, bool overlapped, cudaStream_t stream, Args&&... args)
 {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);
     config.stream = stream;
-    cudaLaunchAttribute attribute[1];
+    cudaLaunchAttribute attribute[2];
     attribute[0].id = cudaLaunchAttributeClusterDimension;
     attribute[0].val.clusterDim.x = ctas;
     attribute[0].val.clusterDim.y = 1;
     attribute[0].val.clusterDim.z = 1;
+    attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[1].val.programmaticStreamSerializationAllowed = overlapped && pdl_enabled() ? 1 : 0;
     config.attrs = attribute;
-    config.numAttrs = 1;
+    config.numAttrs = 2;
     return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
 }
 
