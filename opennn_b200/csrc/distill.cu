@@ -4,7 +4,6 @@
 //   q = softmax over the valid places of u / T     p = softmax(x / T)     p1 = softmax(x)
 //   soft = T^2 sum_k q_k (log q_k - log p_{id_k})   hard = -log(p1_target + FLT_EPSILON)
 //   dx_i = [ soft_weight T (p_i - sum over k with id_k = i of q_k) + hard_weight (p1_i - 1[i = target]) ] / #active
-#include <cooperative_groups.h>
 #include <float.h>
 
 #include "logit_rows.cuh"
@@ -15,164 +14,15 @@ namespace onn
 namespace
 {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-
 __device__ __forceinline__ float finite_anchor(float m) { return m > -INFINITY ? m : 0.f; }
 
-// What a row's softmaxes come to: p_i = 2^((x_i - m) c) * inv and p1_i = 2^((x_i - m) log2 e) * inv1.
-struct Softmaxes
-{
-    float m, c, inverse_temperature, s, s1;
-    __device__ __forceinline__ float p(float x) const { return s > 0.f || s != s ? exp2_approx((x - m) * c) / s : 0.f; }
-    __device__ __forceinline__ float p1(float x) const { return s1 > 0.f || s1 != s1 ? exp2_approx((x - m) * kLog2E) / s1 : 0.f; }
-    __device__ __forceinline__ float log_p(float x) const { return s == 0.f ? -INFINITY : (x - m) * inverse_temperature - logf(s); }
-};
-
-// The teacher's distribution over the places of its list, in shared memory: q[k] (0 for a place that is not valid) and
-// the first place k' <= k with the same id.  Called by the whole CTA; returns whether there is any.
-struct Teacher
-{
-    float q[ONN_TOP_MAX];
-    int id[ONN_TOP_MAX];
-    float reduce[kWarps];
-};
-
-__device__ __forceinline__ float cta_max(float v, float* scratch)
-{
-    v = warp_max(v);
-    __syncthreads();
-    if((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[0];
-#pragma unroll
-    for(int w = 1; w < kWarps; w++) v = fmaxf(v, scratch[w]);
-    return v;
-}
-
-__device__ __forceinline__ float cta_sum(float v, float* scratch)
-{
-    v = warp_sum(v);
-    __syncthreads();
-    if((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for(int w = 0; w < kWarps; w++) v += scratch[w];
-    return v;
-}
-
-// Rows longer than a cluster can hold: one CTA per row, which sweeps it three times.
-template <int DTYPE>
-__global__ void __launch_bounds__(kThreads)
-distill3d_sweeps_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, const float* __restrict__ targets,
-                 const float* __restrict__ active_count, const int* __restrict__ teacher_ids, const float* __restrict__ teacher_logits,
-                 int top, float inverse_temperature, float temperature, float soft_weight, float hard_weight,
-                 typename Logit<DTYPE>::type* dlogits, long long d_pitch, float* __restrict__ row_losses, long long rows, int V)
-{
-    using L = Logit<DTYPE>;
-    __shared__ Teacher teacher;
-    const long long row = blockIdx.x;
-    const int tid = threadIdx.x;
-    const typename L::type* x = logits + row * pitch;
-    typename L::type* dx = dlogits ? dlogits + row * d_pitch : nullptr;
-    bool active;
-    const long long target = row_token(targets, row, V, &active);
-    if(!active)
-    {
-        if(dx) for(int i = tid; i < V; i += kThreads) L::put(dx + i, 0.f);
-        if(tid == 0) { row_losses[row] = 0.f; row_losses[rows + row] = 0.f; }
-        return;
-    }
-
-    // the teacher
-    float u = -INFINITY;
-    int id = -1;
-    if(tid < top)
-    {
-        id = teacher_ids[row * top + tid];
-        if(id < 0 || id >= V) id = -1;
-        else u = teacher_logits[row * top + tid];
-    }
-    const float u_max = cta_max(u, teacher.reduce);
-    // NaN passes the maximum by: it comes in through the sum
-    const float e = id < 0 ? 0.f : exp2_approx((u - finite_anchor(u_max)) * (kLog2E * inverse_temperature));
-    const float e_sum = cta_sum(e, teacher.reduce);
-    const bool taught = e_sum != 0.f;                    // some place is valid and not -inf
-    const float q = taught && id >= 0 ? e / e_sum : 0.f;
-    if(tid < ONN_TOP_MAX) { teacher.q[tid] = q; teacher.id[tid] = id; }
-    __syncthreads();
-
-    // the student's softmaxes
-    float m = -INFINITY;
-    for(int i = tid; i < V; i += kThreads) m = fmaxf(m, L::get(x + i));
-    Softmaxes f;
-    f.m = finite_anchor(cta_max(m, teacher.reduce));
-    f.inverse_temperature = inverse_temperature;
-    f.c = kLog2E * inverse_temperature;
-    float s = 0.f, s1 = 0.f;
-    for(int i = tid; i < V; i += kThreads)
-    {
-        const float d = L::get(x + i) - f.m;
-        s += exp2_approx(d * f.c);
-        s1 += exp2_approx(d * kLog2E);
-    }
-    f.s = cta_sum(s, teacher.reduce);
-    f.s1 = cta_sum(s1, teacher.reduce);
-
-    float term = 0.f;
-    if(taught && id >= 0 && q != 0.f)
-        term = q * ((u - finite_anchor(u_max)) * inverse_temperature - logf(e_sum) - f.log_p(L::get(x + id)));
-    term = cta_sum(term, teacher.reduce);
-    if(tid == 0)
-    {
-        row_losses[row] = term * temperature * temperature;
-        row_losses[rows + row] = hard_weight != 0.f ? -logf(f.p1(L::get(x + target)) + FLT_EPSILON) : 0.f;
-    }
-    if(!dx) return;
-
-    const float count = active_count[0];
-    const float scale = count > 0.f ? 1.f / count : 0.f;
-    const float soft = taught ? soft_weight * temperature * scale : 0.f, hard = hard_weight * scale;
-    // the elements that the list or the target singles out: their student logits, before the gradient takes their place
-    float special = 0.f;
-    int special_index = -1;
-    if(tid <= top)
-    {
-        // one thread for each place of the list, the one after the last place for the target; an index that stands in
-        // several places is done by the first of them
-        special_index = tid < top ? id : (int)target;
-        float q_there = 0.f;
-        for(int k = 0; k < top; k++)
-        {
-            if(teacher.id[k] != special_index || special_index < 0) continue;
-            if(k < tid) { special_index = -1; break; }
-            q_there += teacher.q[k];
-        }
-        if(special_index >= 0)
-        {
-            const float there = L::get(x + special_index);
-            special = soft * (f.p(there) - q_there) + (hard != 0.f ? hard * (f.p1(there) - (special_index == target ? 1.f : 0.f)) : 0.f);
-        }
-    }
-    __syncthreads();
-    for(int i = tid; i < V; i += kThreads)
-    {
-        const float value = L::get(x + i);
-        L::put(dx + i, soft * f.p(value) + (hard != 0.f ? hard * f.p1(value) : 0.f));
-    }
-    __syncthreads();
-    if(special_index >= 0) L::put(dx + special_index, special);
-}
-
-constexpr int kMaxCluster = 8;
 constexpr int kCountInside = 2048;                // up to so many rows a CTA counts the active ones itself
 
-struct alignas(16) Part { float m, s, s1, unused; };
+struct Part { float m, s, s1; };
 
-struct Held
+struct Shared
 {
-    Part parts[kMaxCluster * 32];
+    Part parts[32];
     float q[ONN_TOP_MAX];
     float log_q[ONN_TOP_MAX];
     alignas(16) int id[ONN_TOP_MAX];
@@ -181,29 +31,21 @@ struct Held
     float count[32];
 };
 
-// One cluster of CTAs (often of one) per row, which holds the row in its registers: each logit is read from global memory
-// once, and its gradient written once.  N vectors of 16 bytes per thread.
-//   1  the loads, with the teacher's list under way beside them (one warp does its softmax in each CTA);
-//   2  sums relative to each thread's largest logit, joined over the warp, and put into every CTA's shared memory;
-//   3  the row's maximum and sums, then the gradient from the registers: with one softmax in fp32 (SETS = 1: the
-//      temperature is 1 or there is no hard-label part) the exponentials are kept, else they are formed again;
-//   4  the elements that the list or the target singles out are written again by one thread each.
+// One CTA per row, two sweeps: sums relative to the largest logit on the way up, the gradient on the way down, so that what was
+// read last, and is still in L1, is read again first; the rest comes from L2, which holds the rows that the GPU works on.
 template <int DTYPE, int SETS, int T, int N>
 __global__ void __launch_bounds__(T, 1024 / T)
 distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, const float* __restrict__ targets,
-                 const float* active_count, const int* __restrict__ teacher_ids, const float* __restrict__ teacher_logits,
-                 int top, float inverse_temperature, float temperature, float soft_weight, float hard_weight,
-                 typename Logit<DTYPE>::type* dlogits, long long d_pitch, float* __restrict__ row_losses, long long rows, int V)
+                     const float* active_count, const int* __restrict__ teacher_ids, const float* __restrict__ teacher_logits,
+                     int top, float inverse_temperature, float temperature, float soft_weight, float hard_weight,
+                     typename Logit<DTYPE>::type* dlogits, long long d_pitch, float* __restrict__ row_losses, long long rows, int V)
 {
     using L = Logit<DTYPE>;
     constexpr int VE = L::VE, kWarpsHere = T / 32;
-    constexpr bool kKeep = DTYPE == ONN_F32 && SETS == 1;
-    __shared__ Held held;
+    __shared__ Shared shared;
     pdl_launch_dependents();
     pdl_wait();
-    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const long long row = blockIdx.x / ctas;
+    const long long row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const typename L::type* x = logits + row * pitch;
     typename L::type* dx = dlogits ? dlogits + row * d_pitch : nullptr;
@@ -213,9 +55,7 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
     const RowCut cut = cut_row<DTYPE>(x, V);
     const uint4* body = reinterpret_cast<const uint4*>(x + cut.head);
     const int after = cut.head + cut.vectors * VE;
-    const int end_index = rank != 0 ? -1 : tid < cut.head ? tid : tid < cut.head + cut.tail ? after + tid - cut.head : -1;
-    const int share = (cut.vectors + ctas - 1) / ctas;
-    const int begin = min(rank * share, cut.vectors), end = min(begin + share, cut.vectors);
+    const int end_index = tid < cut.head ? tid : tid < cut.head + cut.tail ? after + tid - cut.head : -1;
     const bool together = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
     auto store = [&](int vector, const float (&f)[VE])
     {
@@ -227,42 +67,24 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
             for(int e = 0; e < VE; e++) L::put(to + e, f[e]);
         }
     };
-
-    if(!active)                                        // the same for the whole cluster
+    if(!active)
     {
         if(dx)
         {
             const float zeros[VE] = {};
-            for(int i = begin + tid; i < end; i += T) store(i, zeros);
+            for(int i = tid; i < cut.vectors; i += T) store(i, zeros);
             if(end_index >= 0) L::put(dx + end_index, 0.f);
         }
-        if(rank == 0 && tid == 0) { row_losses[row] = 0.f; row_losses[rows + row] = 0.f; }
+        if(tid == 0) { row_losses[row] = 0.f; row_losses[rows + row] = 0.f; }
         return;
     }
-    // all CTAs of the cluster must be running before one writes into another: waited for below, under the loads
-    if(ctas > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
-
-    // ---- 1
-    uint4 v[N];
-#pragma unroll
-    for(int u = 0; u < N; u++)
-    {
-        const int i = begin + u * T + tid;
-        v[u] = i < end ? __ldcs(body + i) : L::lowest();
-    }
-    const float end_value = end_index >= 0 ? L::get(x + end_index) : -INFINITY;
-    // thread k < top looks after place k of the list, thread `top` after the target: the logit there, if this CTA needs it
+    // thread k < top looks after place k of the list, thread `top` after the target
     int index = -1;
     if(tid < top) index = __ldg(teacher_ids + row * top + tid);
     else if(tid == top) index = (int)target;
     if(index < 0 || index >= V) index = -1;
-    bool mine = false;                                 // the element is one of this CTA's
-    if(index >= 0)
-    {
-        const int vector = index < cut.head || index >= after ? -1 : (index - cut.head) / VE;
-        mine = vector < 0 ? rank == 0 : vector >= begin && vector < end;
-    }
-    const float special_logit = mine || (rank == 0 && index >= 0) ? L::get(x + index) : -INFINITY;
+    const float special_logit = index >= 0 ? L::get(x + index) : -INFINITY;
+    const float end_value = end_index >= 0 ? L::get(x + end_index) : -INFINITY;
 
     if(warp == 0)
     {
@@ -294,11 +116,11 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
         for(int k = 0; k < kPlaces; k++)
         {
             const int at = k * 32 + lane;
-            held.id[at] = id[k];
-            held.q[at] = sum != 0.f && id[k] >= 0 ? e[k] * inverse : 0.f;
-            held.log_q[at] = (u[k] - largest) * inverse_temperature - log_sum;
+            shared.id[at] = id[k];
+            shared.q[at] = sum != 0.f && id[k] >= 0 ? e[k] * inverse : 0.f;
+            shared.log_q[at] = (u[k] - largest) * inverse_temperature - log_sum;
         }
-        if(lane == 0) held.taught = sum != 0.f;
+        if(lane == 0) shared.taught = sum != 0.f;
     }
     float counted = 0.f;
     if(!active_count)
@@ -309,17 +131,35 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
             counted += t > 0 && t < V ? 1.f : 0.f;
         }
         counted = warp_sum(counted);
-        if(lane == 0) held.count[warp] = counted;
+        if(lane == 0) shared.count[warp] = counted;
     }
 
-    // ---- 2
+    // ---- up
     const float c = kLog2E * inverse_temperature;
     float m = end_value > -INFINITY ? end_value : -INFINITY;
-#pragma unroll
-    for(int u = 0; u < N; u++) m = fmaxf(m, L::max(v[u]));
-    const float base = finite_anchor(m);
-    float s, s1 = 0.f;
+    float s = 0.f, s1 = 0.f;
+    if(end_index >= 0) { s = exp2_approx((end_value - finite_anchor(m)) * c); s1 = exp2_approx((end_value - finite_anchor(m)) * kLog2E); }
+    const int batches = (cut.vectors + T * N - 1) / (T * N);
+    for(int batch = 0; batch < batches; batch++)
     {
+        uint4 v[N];
+        float larger = m;
+#pragma unroll
+        for(int u = 0; u < N; u++)
+        {
+            const int i = (batch * N + u) * T + tid;
+            v[u] = i < cut.vectors ? body[i] : L::lowest();
+        }
+#pragma unroll
+        for(int u = 0; u < N; u++) larger = fmaxf(larger, L::max(v[u]));
+        if(larger > m)
+        {
+            const float down = m > -INFINITY ? m - larger : -INFINITY;
+            s *= exp2_approx(down * c);
+            if(SETS == 2) s1 *= exp2_approx(down * kLog2E);
+            m = larger;
+        }
+        const float base = finite_anchor(m);
         const float2 minus = make_float2(-base, -base), c2 = make_float2(c, c), c1 = make_float2(kLog2E, kLog2E);
         float2 s2 = make_float2(0.f, 0.f), s12 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -331,24 +171,16 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
             for(int e = 0; e < VE; e += 2)
             {
                 const float2 d = add2(make_float2(f[e], f[e + 1]), minus), d2 = mul2(d, c2);
-                const float2 p = make_float2(exp2_approx(d2.x), exp2_approx(d2.y));
-                s2 = add2(s2, p);
-                if(kKeep) { f[e] = p.x; f[e + 1] = p.y; }
+                s2 = add2(s2, make_float2(exp2_approx(d2.x), exp2_approx(d2.y)));
                 if(SETS == 2)
                 {
                     const float2 d1 = mul2(d, c1);
                     s12 = add2(s12, make_float2(exp2_approx(d1.x), exp2_approx(d1.y)));
                 }
             }
-            if(kKeep) v[u] = L::pack(f);
         }
-        s = s2.x + s2.y;
-        s1 = s12.x + s12.y;
-        if(end_index >= 0)
-        {
-            s += exp2_approx((end_value - base) * c);
-            if(SETS == 2) s1 += exp2_approx((end_value - base) * kLog2E);
-        }
+        s += s2.x + s2.y;
+        s1 += s12.x + s12.y;
     }
     const float warp_m = warp_max(m);
     {
@@ -356,36 +188,15 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
         s = warp_sum(s * exp2_approx(down * c));
         if(SETS == 2) s1 = warp_sum(s1 * exp2_approx(down * kLog2E));
     }
-    const Part part = {warp_m, s, s1, 0.f};
-    const int parts = ctas * kWarpsHere;
-    if(ctas == 1)
+    if(lane == 0) shared.parts[warp] = Part{warp_m, s, s1};
+    __syncthreads();
+    const Part other = lane < kWarpsHere ? shared.parts[lane] : Part{-INFINITY, 0.f, 0.f};
+    const float M = finite_anchor(warp_max(other.m));
     {
-        if(lane == 0) held.parts[warp] = part;
-        __syncthreads();
-    }
-    else
-    {
-        asm volatile("barrier.cluster.wait;" ::: "memory");
-        if(lane < ctas) cluster.map_shared_rank(&held, lane)->parts[rank * kWarpsHere + warp] = part;
-        cluster.sync();
-    }
-
-    // ---- 3
-    float row_m = -INFINITY;
-    for(int i = lane; i < parts; i += 32) row_m = fmaxf(row_m, held.parts[i].m);
-    row_m = warp_max(row_m);
-    const float M = finite_anchor(row_m);
-    s = 0.f;
-    s1 = 0.f;
-    for(int i = lane; i < parts; i += 32)
-    {
-        const Part other = held.parts[i];
         const float down = other.m > -INFINITY ? other.m - M : -INFINITY;
-        s = fmaf(other.s, exp2_approx(down * c), s);
-        if(SETS == 2) s1 = fmaf(other.s1, exp2_approx(down * kLog2E), s1);
+        s = warp_sum(other.s * exp2_approx(down * c));
+        s1 = SETS == 2 ? warp_sum(other.s1 * exp2_approx(down * kLog2E)) : s;
     }
-    s = warp_sum(s);
-    s1 = SETS == 2 ? warp_sum(s1) : s;
     // a student without a finite logit has no distribution: p = 0
     const float inverse = s == 0.f ? 0.f : 1.f / s, inverse1 = s1 == 0.f ? 0.f : 1.f / s1;
     float count = 0.f;
@@ -393,10 +204,10 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
     else
     {
 #pragma unroll
-        for(int w = 0; w < kWarpsHere; w++) count += held.count[w];
+        for(int w = 0; w < kWarpsHere; w++) count += shared.count[w];
     }
     const float scale = count > 0.f ? 1.f / count : 0.f;
-    const bool taught = held.taught != 0;
+    const bool taught = shared.taught != 0;
     const float soft = taught ? soft_weight * temperature * scale : 0.f, hard = hard_weight * scale;
     // one softmax serves both parts at temperature 1
     const float weight = SETS == 2 ? soft * inverse : (soft + hard) * inverse, weight1 = hard * inverse1;
@@ -407,88 +218,92 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
         const float g = weight * exp2_approx((logit - M) * c);
         return SETS == 2 ? fmaf(weight1, exp2_approx((logit - M) * kLog2E), g) : g;
     };
+
+    // ---- down
     if(dx)
     {
-        const float again = (m > -INFINITY ? exp2_approx((m - M) * c) : 0.f) * weight;
         const float2 minus = make_float2(-M, -M), c2 = make_float2(c, c), c1 = make_float2(kLog2E, kLog2E);
-        const float2 again2 = make_float2(again, again), w2 = make_float2(weight, weight), w12 = make_float2(weight1, weight1);
-#pragma unroll
-        for(int u = 0; u < N; u++)
+        const float2 w2 = make_float2(weight, weight), w12 = make_float2(weight1, weight1);
+        for(int batch = batches - 1; batch >= 0; batch--)
         {
-            const int i = begin + u * T + tid;
-            if(i >= end) continue;
-            float f[VE];
-            L::unpack(v[u], f);
+            uint4 v[N];
 #pragma unroll
-            for(int e = 0; e < VE; e += 2)
+            for(int u = 0; u < N; u++)
             {
-                float2 g = make_float2(f[e], f[e + 1]);
-                if(kKeep) g = mul2(g, again2);
-                else
+                const int i = (batch * N + u) * T + tid;
+                if(i < cut.vectors) v[u] = __ldcs(body + i);
+            }
+#pragma unroll
+            for(int u = 0; u < N; u++)
+            {
+                const int i = (batch * N + u) * T + tid;
+                if(i >= cut.vectors) continue;
+                float f[VE];
+                L::unpack(v[u], f);
+#pragma unroll
+                for(int e = 0; e < VE; e += 2)
                 {
-                    const float2 d = add2(g, minus), d2 = mul2(d, c2);
-                    g = mul2(make_float2(exp2_approx(d2.x), exp2_approx(d2.y)), w2);
+                    const float2 d = add2(make_float2(f[e], f[e + 1]), minus), d2 = mul2(d, c2);
+                    float2 g = mul2(make_float2(exp2_approx(d2.x), exp2_approx(d2.y)), w2);
                     if(SETS == 2)
                     {
                         const float2 d1 = mul2(d, c1);
                         g = fma2(make_float2(exp2_approx(d1.x), exp2_approx(d1.y)), w12, g);
                     }
+                    f[e] = g.x;
+                    f[e + 1] = g.y;
                 }
-                f[e] = g.x;
-                f[e + 1] = g.y;
+                store(i, f);
             }
-            store(i, f);
         }
         if(end_index >= 0) L::put(dx + end_index, gradient(end_value));
     }
 
-    // ---- 4
+    // ---- the elements that the list or the target singles out
     float special = 0.f;
+    bool mine = index >= 0;
     if(mine)
     {
         // an index that stands in several places is done by the first of them, the target by its place in the list if it has one
         int equal = 0;
         for(int k = 0; k < top; k += 4)
         {
-            const int4 four = *reinterpret_cast<const int4*>(held.id + k);     // places past the list hold -1
+            const int4 four = *reinterpret_cast<const int4*>(shared.id + k);     // places past the list hold -1
             equal += (four.x == index) + (four.y == index) + (four.z == index) + (four.w == index);
         }
-        float q = tid < top ? held.q[tid] : 0.f;
+        float q = tid < top ? shared.q[tid] : 0.f;
         if(equal > (tid < top ? 1 : 0))
         {
             q = 0.f;
             for(int k = 0; k < top; k++)
             {
-                if(held.id[k] != index) continue;
+                if(shared.id[k] != index) continue;
                 if(k < tid) { mine = false; break; }
-                q += held.q[k];
+                q += shared.q[k];
             }
         }
         special = soft * (p_of(special_logit) - q);
         if(hard != 0.f) special += hard * ((SETS == 2 ? p1_of(special_logit) : p_of(special_logit)) - (index == (int)target ? 1.f : 0.f));
     }
-    if(rank == 0)
+    if(warp < ONN_TOP_MAX / 32)
     {
-        if(warp < ONN_TOP_MAX / 32)
+        float term = 0.f;
+        if(tid < top && index >= 0 && shared.q[tid] != 0.f)
         {
-            float term = 0.f;
-            if(tid < top && index >= 0 && held.q[tid] != 0.f)
-            {
-                const float log_p = s == 0.f ? -INFINITY : (special_logit - M) * inverse_temperature - logf(s);
-                term = held.q[tid] * (held.log_q[tid] - log_p);
-            }
-            term = warp_sum(term);
-            if(lane == 0) held.term[warp] = term;
+            const float log_p = s == 0.f ? -INFINITY : (special_logit - M) * inverse_temperature - logf(s);
+            term = shared.q[tid] * (shared.log_q[tid] - log_p);
         }
-        if(tid == top) row_losses[rows + row] = hard_weight != 0.f ? -logf((SETS == 2 ? p1_of(special_logit) : p_of(special_logit)) + FLT_EPSILON) : 0.f;
+        term = warp_sum(term);
+        if(lane == 0) shared.term[warp] = term;
     }
-    __syncthreads();                                   // the stores of 3 come before those that replace them
+    if(tid == top) row_losses[rows + row] = hard_weight != 0.f ? -logf((SETS == 2 ? p1_of(special_logit) : p_of(special_logit)) + FLT_EPSILON) : 0.f;
+    __syncthreads();                                   // the stores of the sweep come before those that replace them
     if(dx && mine) L::put(dx + index, special);
-    if(rank == 0 && tid == 0)
+    if(tid == 0)
     {
         float term = 0.f;
 #pragma unroll
-        for(int w = 0; w < (kWarpsHere < ONN_TOP_MAX / 32 ? kWarpsHere : ONN_TOP_MAX / 32); w++) term += held.term[w];
+        for(int w = 0; w < (kWarpsHere < ONN_TOP_MAX / 32 ? kWarpsHere : ONN_TOP_MAX / 32); w++) term += shared.term[w];
         row_losses[row] = term * temperature * temperature;
     }
 }
@@ -536,18 +351,8 @@ int launch(const void* logits, int64_t pitch, const float* targets, const float*
            int64_t d_pitch, float* row_losses, float* stats, int64_t rows, int64_t V, cudaStream_t stream)
 {
     using E = typename Logit<DTYPE>::type;
-    // CTAs of a row: as many as hold it at 8 vectors per thread of 256 threads, 512 or 1024 for the longest; more while the GPU
-    // is not full and each has two vectors per thread
-    const int64_t vectors = V / Logit<DTYPE>::VE + 1;
-    int T = 256;
-    while(T < 1024 && vectors > (int64_t)kMaxCluster * T * 8) T *= 2;
-    const bool fits = vectors <= (int64_t)kMaxCluster * T * 8;
-    int ctas = (int)((vectors + T * 8 - 1) / (T * 8));
-    while(ctas < kMaxCluster && rows * ctas < 2 * kSmCount && vectors > (int64_t)ctas * T * 2) ctas++;
-    const int64_t each = (vectors + ctas * T - 1) / (ctas * T);
-
     bool counted = false;
-    if(!active_count && (rows > kCountInside || !fits))
+    if(!active_count && rows > kCountInside)
     {
         distill3d_count_kernel<<<1, 1024, 0, stream>>>(targets, rows, V, stats);
         count_launch();
@@ -555,32 +360,36 @@ int launch(const void* logits, int64_t pitch, const float* targets, const float*
         active_count = stats + 2;
         counted = true;
     }
+    // Threads of a row.  The rows that the GPU works on should stay in L2 (and in part in L1) between the two sweeps, so long rows
+    // want few large CTAs; what a row costs besides its logits is latency, so short ones want many small CTAs.  In us:
+    //                          128     256     512    1024
+    //   16384 x   8000 fp32    210     239     322     591
+    //    8192 x  32000 fp32    454     393     385     531
+    //    8192 x  50021 fp32    771     679     631     752
+    //    2048 x 131072 fp32            490     454     435
+    //    8192 x  32000 bf16    212     217     266     459
+    //    8192 x  50021 bf16    362     335     384     539
+    //    2048 x 131072 bf16            241     218     256
+    // With less than two rows for each SM nothing is gained by small CTAs.
+    const int64_t vectors = V / Logit<DTYPE>::VE;
+    const bool wide = DTYPE == ONN_F32;
+    int T = vectors >= (wide ? 24576 : 49152) ? 1024 : vectors >= (wide ? 6144 : 10240) ? 512 : vectors >= 4000 || top >= 128 ? 256 : 128;
+    while(T < 1024 && rows * T <= 512 * kSmCount && vectors >= 4 * T) T *= 2;
+
     const E* x = static_cast<const E*>(logits);
     E* dx = static_cast<E*>(dlogits);
-    const float inverse_temperature = 1.f / temperature;
-    cudaError_t error;
-    if(!fits)
+    // at temperature 1 one softmax serves both parts
+    const bool two = hard_weight != 0.f && temperature != 1.f;
+    auto run = [&](auto kernel)
     {
-        distill3d_sweeps_kernel<DTYPE><<<(unsigned)rows, kThreads, 0, stream>>>(
-            x, pitch, targets, active_count, teacher_ids, teacher_logits, (int)top, inverse_temperature, temperature, soft_weight,
-            hard_weight, dx, d_pitch, row_losses, rows, (int)V);
-        error = cudaGetLastError();
-    }
-    else
-    {
-        const bool two = hard_weight != 0.f && temperature != 1.f;
-        auto held = [&](auto kernel)
-        {
-            return launch_clusters(kernel, (unsigned)(rows * ctas), T, ctas, counted, stream, x, (long long)pitch, targets, active_count,
-                                   teacher_ids, teacher_logits, (int)top, inverse_temperature, temperature, soft_weight, hard_weight, dx,
-                                   (long long)d_pitch, row_losses, (long long)rows, (int)V);
-        };
-#define ONN_HELD(SETS) (T == 1024 ? held(distill3d_kernel<DTYPE, SETS, 1024, 8>) : T == 512 ? held(distill3d_kernel<DTYPE, SETS, 512, 8>) : \
-                        each > 4 ? held(distill3d_kernel<DTYPE, SETS, 256, 8>) : each > 2 ? held(distill3d_kernel<DTYPE, SETS, 256, 4>) : \
-                        each > 1 ? held(distill3d_kernel<DTYPE, SETS, 256, 2>) : held(distill3d_kernel<DTYPE, SETS, 256, 1>))
-        error = two ? ONN_HELD(2) : ONN_HELD(1);
-#undef ONN_HELD
-    }
+        return launch_clusters(kernel, (unsigned)rows, T, 1, 0, counted, stream, x, (long long)pitch, targets, active_count, teacher_ids,
+                               teacher_logits, (int)top, 1.f / temperature, temperature, soft_weight, hard_weight, dx, (long long)d_pitch,
+                               row_losses, (long long)rows, (int)V);
+    };
+    const cudaError_t error = T == 1024 ? (two ? run(distill3d_kernel<DTYPE, 2, 1024, 8>) : run(distill3d_kernel<DTYPE, 1, 1024, 8>))
+                            : T == 512 ? (two ? run(distill3d_kernel<DTYPE, 2, 512, 8>) : run(distill3d_kernel<DTYPE, 1, 512, 8>))
+                            : T == 256 ? (two ? run(distill3d_kernel<DTYPE, 2, 256, 8>) : run(distill3d_kernel<DTYPE, 1, 256, 8>))
+                                       : (two ? run(distill3d_kernel<DTYPE, 2, 128, 4>) : run(distill3d_kernel<DTYPE, 1, 128, 4>));
     count_launch();
     if(error != cudaSuccess) return ONN_ERR_CUDA;
     return launch_status();

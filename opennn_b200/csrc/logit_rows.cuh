@@ -190,11 +190,12 @@ __device__ __forceinline__ long long row_token(const float* tokens, long long ro
 
 // A launch in clusters of `ctas` CTAs.  overlapped: as launch_overlapped (the kernel calls pdl_wait first).
 template <typename... KernelArgs, typename... Args>
-inline cudaError_t launch_clusters(void (*kernel)(KernelArgs...), unsigned int grid, int threads, int ctas, bool overlapped, cudaStream_t stream, Args&&... args)
+inline cudaError_t launch_clusters(void (*kernel)(KernelArgs...), unsigned int grid, int threads, int ctas, size_t dynamic_bytes, bool overlapped, cudaStream_t stream, Args&&... args)
 {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = dynamic_bytes;
     config.stream = stream;
     cudaLaunchAttribute attribute[2];
     attribute[0].id = cudaLaunchAttributeClusterDimension;

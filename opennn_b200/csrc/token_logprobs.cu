@@ -643,7 +643,7 @@ int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float*
     // whoever is free takes the next (203 us against 213 for 8192 rows of 50021 with 64 alternatives)
     int64_t clusters = rows;
     if(T == 32 && clusters > 24 * kSmCount) clusters = 24 * kSmCount;
-    if(launch_clusters(token_logprobs_kernel<DTYPE, TOP, T, N>, (unsigned)(clusters * ctas), T, ctas, false, stream,
+    if(launch_clusters(token_logprobs_kernel<DTYPE, TOP, T, N>, (unsigned)(clusters * ctas), T, ctas, 0, false, stream,
                        static_cast<const typename L::type*>(logits), (long long)pitch, tokens, logprobs, entropy, lse, top_ids,
                        top_logprobs, (int)top, (long long)rows, (int)V, c, inverse_temperature) != cudaSuccess) return ONN_ERR_CUDA;
     count_launch();
