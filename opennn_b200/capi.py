@@ -196,8 +196,8 @@ def _current_stream(t):
 
 
 def embedding_bwd_sorted(ids, dY, V, scale=True, dY2=None, dW=None, accumulate=False):
-    """embedding_bwd with the rows of each token added in order of position.  dW [V, E] is written (a new tensor if None),
-    or added to with accumulate=True."""
+    """embedding_bwd with the rows of each token added in a fixed order.  dW [V, E] is written (a new tensor if None), or added
+    to with accumulate=True."""
     B, S, E = dY.shape
     if dW is None:
         dW = (torch.zeros if accumulate else torch.empty)(V, E, device="cuda")
