@@ -196,7 +196,7 @@ int onn_embedding_bwd(const float* ids, const float* dY, const float* dY2, float
  * The order of the additions depends on B * S and the ids alone.  Nothing is added atomically, so frequent tokens do
  * not contend (onn_embedding_bwd adds each position's row with fp32 reductions in whatever order they arrive).
  * flags 0: all of dW [V, E] is overwritten, with zeros for row 0 and for tokens that do not occur; ONN_ACCUMULATE: added
- * to the rows of the tokens that do, the others are left alone.  E < 2^23, V < 2^24, B * S < 2^31 - 65536.
+ * to the rows of the tokens that do, the others are left alone.  E, V < 2^23, B * S < 2^31 - 65536.
  * workspace: onn_embedding_bwd_sorted_workspace_floats floats, 16-byte aligned (may be NULL when that is 0); calls that
  * can overlap on the GPU need one each. */
 size_t onn_embedding_bwd_sorted_workspace_floats(int64_t B, int64_t S, int64_t E, int64_t V);

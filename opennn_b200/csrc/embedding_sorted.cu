@@ -2,16 +2,17 @@
 //   dW[v, :] (+)= sqrt(E) * sum over the positions n with id v of (dY + dY2)[n, :],   0 < v < V.
 // No atomics on floating-point values: the same inputs give the same bits.
 //
-// Bound by HBM: every gradient row is read once and every table row written once.  Three launches:
-//   1  one cluster sorts the positions by id (stable radix sort, its passes joined by cluster barriers), while the other
-//      clusters mark the ids that occur in their part of the table and write the zeros of the rows that do not;
+// Bound by HBM: every gradient row is read once and every table row written once.
+//   1  the positions are sorted by id.  CTA c has every P-th row of the table from the c-th on (neighbouring ids are often
+//      frequent together): it reads all ids, keeps the positions of its own, counts those of the CTAs before it, which
+//      tells where its part of the sorted list begins, and sorts what it has kept.  No CTA needs another's result, so one
+//      launch does it: 6.5 us for 16384 positions (a radix sort by one cluster, or in launches of counts and places: 14 to
+//      20).  The same CTA writes the zeros of its rows that do not occur;
 //   2  the sorted positions are cut into equal chunks, whatever their ids, so that a frequent token is spread over many
 //      CTAs; a group of threads adds the rows of a chunk, and writes the table row of each run of equal ids that lies inside it.
 //      Runs that cross the edge of a chunk leave a partial sum;
-//   3  the partial sums of each such run are added in order.
+//   3  the partial sums of each run that crosses an edge are added in order.
 // Few positions take one launch instead: every CTA owns some rows of the table and looks for their ids itself.
-#include <cooperative_groups.h>
-
 #include "common.cuh"
 #include "launch_counter.h"
 
@@ -21,8 +22,6 @@ namespace onn
 namespace
 {
 
-namespace cg = cooperative_groups;
-
 // ---------------------------------------------------------------------------------------
 // Few positions
 // ---------------------------------------------------------------------------------------
@@ -30,24 +29,28 @@ namespace cg = cooperative_groups;
 constexpr int kOwnerThreads = 256;
 constexpr int kOwnerWarps = kOwnerThreads / 32;
 constexpr int kTile = 1024;                       // ids looked at together
-constexpr int kOwnerColumns = 256;                // one per thread
+constexpr int kOwnerColumns = 64;
+constexpr int kOwnerGroups = kOwnerThreads / kOwnerColumns;
+constexpr int kOwnerInFlight = 8;                 // gradient elements a thread has under way
 constexpr int kMaxOwned = 32;                     // rows of a CTA, summed in shared memory
 
-// CTA (x, y) owns `owned` consecutive rows of the table, 256 columns of them.  It walks over all ids in order, keeps those that
-// are its own (in order: prefix sums) and adds their gradient rows; a thread always has the same column.
+// CTA (x, y) owns `owned` consecutive rows of the table, 64 columns of them.  It walks over all ids in order and keeps those that
+// are its own (in order: prefix sums); four groups of 64 threads, one per column, add every fourth of their gradient
+// rows each, and the groups' sums are added in order.
 __global__ void __launch_bounds__(kOwnerThreads)
 embedding_owner_kernel(const float* __restrict__ ids, const float* __restrict__ dY, const float* __restrict__ dY2,
                        float* __restrict__ dW, int tokens, int E, int V, float scale, int owned, int accumulate)
 {
-    __shared__ float sums[kMaxOwned][kOwnerColumns];
+    __shared__ float sums[kOwnerGroups][kMaxOwned][kOwnerColumns];
     __shared__ unsigned char present[kMaxOwned];
-    __shared__ int list_row[kTile];
-    __shared__ int list_token[kTile];
+    __shared__ unsigned short list_row[kTile];
+    __shared__ unsigned short list_token[kTile];
     __shared__ int warp_count[kOwnerWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = tid / kOwnerColumns, in_group = tid % kOwnerColumns;
     const int v0 = blockIdx.x * owned, v1 = min(v0 + owned, V);
-    const int column = blockIdx.y * kOwnerColumns + tid;
-    for(int r = 0; r < owned; r++) sums[r][tid] = 0.f;
+    const int column = blockIdx.y * kOwnerColumns + in_group;
+    for(int r = 0; r < owned; r++) sums[group][r][in_group] = 0.f;
     if(tid < kMaxOwned) present[tid] = 0;
     for(int first = 0; first < tokens; first += kTile)
     {
@@ -84,36 +87,45 @@ embedding_owner_kernel(const float* __restrict__ ids, const float* __restrict__ 
         for(int k = 0; k < kEach; k++)
         {
             if(found[k] < 0) continue;
-            list_row[before] = found[k];
-            list_token[before] = first + tid * kEach + k;
+            list_row[before] = (unsigned short)found[k];
+            list_token[before] = (unsigned short)(tid * kEach + k);
             present[found[k]] = 1;
             before++;
         }
         __syncthreads();
         if(column < E)
         {
-            for(int i = 0; i < total; i += 4)
+            for(int i = group; i < total; i += kOwnerGroups * kOwnerInFlight)
             {
-                float g[4];
+                float g[kOwnerInFlight];
 #pragma unroll
-                for(int k = 0; k < 4; k++)
+                for(int k = 0; k < kOwnerInFlight; k++)
                 {
-                    const long long at = i + k < total ? (long long)list_token[i + k] * E + column : -1;
-                    g[k] = at >= 0 ? __ldg(dY + at) : 0.f;
-                    if(dY2 && at >= 0) g[k] += __ldg(dY2 + at);
+                    const int j = i + k * kOwnerGroups;
+                    g[k] = 0.f;
+                    if(j >= total) continue;
+                    const long long at = (long long)(first + list_token[j]) * E + column;
+                    g[k] = __ldg(dY + at);
+                    if(dY2) g[k] += __ldg(dY2 + at);
                 }
 #pragma unroll
-                for(int k = 0; k < 4; k++)
-                    if(i + k < total) sums[list_row[i + k]][tid] += g[k];
+                for(int k = 0; k < kOwnerInFlight; k++)
+                {
+                    const int j = i + k * kOwnerGroups;
+                    if(j < total) sums[group][list_row[j]][in_group] += g[k];
+                }
             }
         }
     }
     __syncthreads();
     if(column >= E) return;
-    for(int v = v0; v < v1; v++)
+    for(int v = v0 + group; v < v1; v += kOwnerGroups)
     {
         float* to = dW + (long long)v * E + column;
-        const float sum = sums[v - v0][tid] * scale;
+        float sum = sums[0][v - v0][in_group];
+#pragma unroll
+        for(int q = 1; q < kOwnerGroups; q++) sum += sums[q][v - v0][in_group];
+        sum *= scale;
         if(!accumulate) *to = sum;
         else if(present[v - v0]) *to += sum;
     }
@@ -123,174 +135,212 @@ embedding_owner_kernel(const float* __restrict__ ids, const float* __restrict__ 
 // 1: sort, and the zeros
 // ---------------------------------------------------------------------------------------
 
-constexpr int kSortCtas = 8;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kMaxDigitBits = 9;
-constexpr int kMaxBins = 1 << kMaxDigitBits;
-constexpr int kZeroClusters = 17;                 // 18 clusters of 8: 144 of the 148 SMs
+constexpr int kMinParts = 128;                    // CTAs: a power of two
+constexpr int kMaxRows = 512;                     // of the table, a CTA's part
+constexpr int kRowBits = 9;
+constexpr int kList = 512;                        // positions that a warp keeps; beyond that it reads the ids again
 
 struct SortShared
 {
-    unsigned int count[kSortWarps][kMaxBins];     // of each warp's positions: digits seen; then where its next one goes
-    unsigned int total[kSortCtas][kMaxBins];      // written by every CTA of the cluster
-    unsigned int base[kMaxBins];
-    unsigned int warp_sum[kMaxBins / 32];
+    unsigned int count[kSortWarps][kMaxRows];     // of each warp: how often a row occurs; then where its next position goes
+    unsigned int position[kSortWarps][kList];
+    unsigned short row[kSortWarps][kList];
+    unsigned int warp_sum[kSortWarps];
+    unsigned int warp_lower[kSortWarps];
+    unsigned char present[kMaxRows];
 };
 
-__device__ __forceinline__ unsigned int sort_key(const float* __restrict__ ids, long long n, unsigned int V)
+// The lanes of the warp whose row is this lane's: one vote per bit.
+__device__ __forceinline__ unsigned int lanes_with(unsigned int row, bool there)
 {
-    const long long v = token_index(__ldg(ids + n));
-    return v > 0 && v < (long long)V ? (unsigned int)v : V;         // V: padding, sorted behind everything
+    unsigned int same = __ballot_sync(0xffffffffu, there);
+#pragma unroll
+    for(int b = 0; b < kRowBits; b++)
+    {
+        const unsigned int set = __ballot_sync(0xffffffffu, (row >> b) & 1u);
+        same &= (row >> b) & 1u ? set : ~set;
+    }
+    return same;
 }
 
-__device__ void sort_by_id(SortShared& shared, const float* __restrict__ ids, uint2* buffer0, uint2* buffer1, int tokens, unsigned int V,
-                           int passes, int digit_bits, cg::cluster_group& cluster)
+// CTA c has the rows v of the table with (v - 1) % parts = c, parts = 1 << part_bits; its row r is v = (r << part_bits) + c + 1.
+// (The last CTA has row 0 as well, which no position has.)  Warp w looks at the w-th of 32 equal stretches of the ids.
+__global__ void __launch_bounds__(kSortThreads, 1)
+embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted, int* __restrict__ control, float* __restrict__ dW,
+                      int tokens, int E, int V, int part_bits, int write_zeros)
 {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank();
-    const int bins = 1 << digit_bits;
-    // warp w of CTA r has positions [from, to): in order of warp, so the sort is stable
-    const int warps = kSortCtas * kSortWarps;
-    const int each = ((tokens + warps - 1) / warps + 31) & ~31;
-    const long long begin = (long long)(rank * kSortWarps + warp) * each;
-    const int from = (int)(begin < tokens ? begin : tokens), to = (int)(begin + each < tokens ? begin + each : tokens);
-    cluster.sync();                                                  // every CTA is running: its shared memory may be written
-    for(int pass = 0; pass < passes; pass++)
+    extern __shared__ __align__(16) unsigned char bytes[];
+    SortShared& shared = *reinterpret_cast<SortShared*>(bytes);
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned int below = (1u << lane) - 1u;
+    const unsigned int part = blockIdx.x, part_mask = (1u << part_bits) - 1u;
+    const int rows = V - 1 > (int)part ? ((V - 2 - (int)part) >> part_bits) + 1 : 0;
+    constexpr int kBlock = 512;                       // ids a warp looks at together, 16 neighbouring ones per lane
+    const long long stretch = ((tokens + kSortWarps - 1) / kSortWarps + kBlock - 1) / kBlock * kBlock;
+    const long long from = warp * stretch < tokens ? warp * stretch : tokens, to = from + stretch < tokens ? from + stretch : tokens;
+    const bool vec = aligned16(ids);
+    unsigned int* const count = shared.count[warp];
+    unsigned int* const list_position = shared.position[warp];
+    unsigned short* const list_row = shared.row[warp];
+    for(int r = lane; r < rows; r += 32) count[r] = 0;
+
+    // found(n of the lane's first id, the rows of its ids or -1, how many of the warp's lie before the lane's, how many there are)
+    unsigned int lower = 0;
+    auto scan = [&](auto found)
     {
-        const int shift = pass * digit_bits;
-        const uint2* source = (pass & 1) ? buffer0 : buffer1;        // of passes after the first
-        uint2* destination = (pass & 1) ? buffer1 : buffer0;
-        unsigned int* count = shared.count[warp];
-        for(int b = lane; b < bins; b += 32) count[b] = 0;
-        __syncwarp();
-        auto item = [&](int n)
+        for(long long first = from; first < to; first += kBlock)
         {
-            if(n >= to) return make_uint2(0xffffffffu, 0u);
-            return pass == 0 ? make_uint2(sort_key(ids, n, V), (unsigned int)n) : __ldcg(source + n);
-        };
-        for(int n = from; n < to; n += 32)
-        {
-            const uint2 it = item(n + lane);
-            const bool there = n + lane < to;
-            const unsigned int digit = there ? (it.x >> shift) & (unsigned int)(bins - 1) : 0xffffu;
-            const unsigned int same = __match_any_sync(0xffffffffu, digit);
-            if(there && lane == __ffs(same) - 1) count[digit] += __popc(same);
-            __syncwarp();
-        }
-        __syncthreads();
-        if(tid < bins)
-        {
-            // where each warp's share of a digit starts inside the CTA's
-            unsigned int run = 0;
-            for(int w = 0; w < kSortWarps; w++)
-            {
-                const unsigned int c = shared.count[w][tid];
-                shared.count[w][tid] = run;
-                run += c;
-            }
-            for(int r = 0; r < kSortCtas; r++) cluster.map_shared_rank(&shared, r)->total[rank][tid] = run;
-        }
-        cluster.sync();
-        unsigned int all = 0, before = 0;
-        if(tid < bins)
-        {
+            const long long n = first + lane * 16;
+            float id[16];
 #pragma unroll
-            for(int r = 0; r < kSortCtas; r++)
+            for(int q = 0; q < 4; q++)
             {
-                if(r < rank) before += shared.total[r][tid];
-                all += shared.total[r][tid];
+                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                const long long at = n + q * 4;
+                if(vec && at + 4 <= to) f = __ldg(reinterpret_cast<const float4*>(ids + at));
+                else
+                {
+                    if(at < to) f.x = __ldg(ids + at);
+                    if(at + 1 < to) f.y = __ldg(ids + at + 1);
+                    if(at + 2 < to) f.z = __ldg(ids + at + 2);
+                    if(at + 3 < to) f.w = __ldg(ids + at + 3);
+                }
+                id[q * 4] = f.x; id[q * 4 + 1] = f.y; id[q * 4 + 2] = f.z; id[q * 4 + 3] = f.w;
             }
-        }
-        unsigned int upto = all;
-        if(tid < kMaxBins)
-        {
+            int row[16], mine = 0;
+#pragma unroll
+            for(int j = 0; j < 16; j++)
+            {
+                // 2^23 + id, rounded toward zero, holds trunc(id) in its low bits for 0 <= id < 2^23; everything else (negative,
+                // larger, NaN) comes out far above V - 1 when 2^23 + 1 is taken from the bits
+                const unsigned int before = __float_as_uint(__fadd_rz(id[j], 8388608.f)) - 0x4b000001u;      // id - 1
+                const bool valid = before < (unsigned int)(V - 1);
+                const unsigned int its = before & part_mask;
+                lower += valid && its < part;
+                row[j] = valid && its == part ? (int)(before >> part_bits) : -1;
+                mine += row[j] >= 0;
+            }
+            if(!__any_sync(0xffffffffu, mine != 0)) continue;
+            int upto = mine;
 #pragma unroll
             for(int offset = 1; offset < 32; offset <<= 1)
             {
-                const unsigned int other = __shfl_up_sync(0xffffffffu, upto, offset);
+                const int other = __shfl_up_sync(0xffffffffu, upto, offset);
                 if(lane >= offset) upto += other;
             }
-            if(lane == 31) shared.warp_sum[warp] = upto;
+            found((unsigned int)n, row, upto - mine, __shfl_sync(0xffffffffu, upto, 31));
         }
-        __syncthreads();
-        if(tid < bins)
-        {
-            unsigned int lower = 0;
-            for(int w = 0; w < warp; w++) lower += shared.warp_sum[w];
-            shared.base[tid] = lower + upto - all + before;
-        }
-        __syncthreads();
-        for(int n = from; n < to; n += 32)
-        {
-            const uint2 it = item(n + lane);
-            const bool there = n + lane < to;
-            const unsigned int digit = there ? (it.x >> shift) & (unsigned int)(bins - 1) : 0xffffu;
-            const unsigned int same = __match_any_sync(0xffffffffu, digit);
-            const unsigned int at = there ? shared.base[digit] + count[digit] + __popc(same & ((1u << lane) - 1u)) : 0u;
-            __syncwarp();
-            if(there)
-            {
-                destination[at] = it;
-                if(lane == __ffs(same) - 1) count[digit] += __popc(same);
-            }
-            __syncwarp();
-        }
-        cluster.sync();                                              // what this pass wrote is there for the next one
-    }
-}
-
-// The rows [v0, v1) of the table that no position has become zero.
-__device__ void zero_absent_rows(unsigned int* present, const float* __restrict__ ids, float* __restrict__ dW, int tokens, int E,
-                                 int v0, int v1)
-{
-    const int tid = threadIdx.x;
-    for(int i = tid; i < (v1 - v0 + 31) / 32; i += kSortThreads) present[i] = 0;
-    __syncthreads();
-#pragma unroll 8
-    for(int n = tid; n < tokens; n += kSortThreads)
+    };
+    auto keep = [&](unsigned int n, const int (&row)[16], int at)
     {
-        const long long v = token_index(__ldg(ids + n));
-        if(v > 0 && v >= v0 && v < v1) atomicOr(present + (int)(v - v0) / 32, 1u << ((int)(v - v0) & 31));
+#pragma unroll
+        for(int j = 0; j < 16; j++)
+        {
+            if(row[j] < 0) continue;
+            if(at < kList) { list_position[at] = n + j; list_row[at] = (unsigned short)row[j]; }
+            at++;
+        }
+    };
+    int kept = 0;
+    scan([&](unsigned int n, const int (&row)[16], int before, int all) { keep(n, row, kept + before); kept += all; });
+    __syncwarp();
+    // the warp's positions in order, 32 at a time: from its list, or from the ids again, 512 of them by way of the list
+    auto each = [&](auto act)
+    {
+        auto from_list = [&](int n)
+        {
+            for(int i = 0; i < n; i += 32)
+            {
+                const bool there = i + lane < n;
+                const unsigned int row = there ? list_row[i + lane] : 0u;
+                act(there, row, there ? list_position[i + lane] : 0u, lanes_with(row, there));
+            }
+        };
+        if(kept <= kList) from_list(kept);
+        else
+        {
+            scan([&](unsigned int n, const int (&row)[16], int before, int all)
+            {
+                keep(n, row, before);
+                __syncwarp();
+                from_list(all);
+                __syncwarp();
+            });
+        }
+    };
+    const unsigned int lower_of_warp = __reduce_add_sync(0xffffffffu, lower);
+    if(lane == 0) shared.warp_lower[warp] = lower_of_warp;
+    each([&](bool there, unsigned int row, unsigned int, unsigned int same)
+    {
+        if(there && (same & below) == 0) count[row] += __popc(same);
+        __syncwarp();
+    });
+    __syncthreads();
+
+    // thread r: where each warp's share of row r goes
+    unsigned int all = 0;
+    if(tid < rows)
+    {
+#pragma unroll 8
+        for(int w = 0; w < kSortWarps; w++) all += shared.count[w][tid];
+        shared.present[tid] = all != 0;
+    }
+    unsigned int upto = all;
+#pragma unroll
+    for(int offset = 1; offset < 32; offset <<= 1)
+    {
+        const unsigned int other = __shfl_up_sync(0xffffffffu, upto, offset);
+        if(lane >= offset) upto += other;
+    }
+    if(lane == 31) shared.warp_sum[warp] = upto;
+    __syncthreads();
+    unsigned int start = __reduce_add_sync(0xffffffffu, shared.warp_lower[lane] + (lane < warp ? shared.warp_sum[lane] : 0u)) + upto - all;
+    if(tid == kSortThreads - 1 && blockIdx.x == gridDim.x - 1) { control[0] = 0; control[1] = 0; control[2] = (int)(start + all); }
+    if(tid < rows)
+    {
+#pragma unroll 8
+        for(int w = 0; w < kSortWarps; w++)
+        {
+            const unsigned int c = shared.count[w][tid];
+            shared.count[w][tid] = start;
+            start += c;
+        }
     }
     __syncthreads();
-    const bool vec = (E & 3) == 0 && aligned16(dW);
+    each([&](bool there, unsigned int row, unsigned int position, unsigned int same)
+    {
+        const unsigned int at = there ? count[row] + __popc(same & below) : 0u;
+        __syncwarp();
+        if(there) sorted[at] = make_uint2((row << part_bits) + part + 1u, position);
+        if(there && (same & below) == 0) count[row] += __popc(same);
+        __syncwarp();
+    });
+
+    if(!write_zeros) return;
+    const bool vec_rows = (E & 3) == 0 && aligned16(dW);
+    auto zero = [&](int v)
+    {
+        float* to_row = dW + (long long)v * E;
+        if(vec_rows) for(int e = lane * 4; e < E; e += 128) st4(to_row + e, make_float4(0.f, 0.f, 0.f, 0.f));
+        else for(int e = lane; e < E; e += 32) to_row[e] = 0.f;
+    };
+    if(part == part_mask && warp == 0) zero(0);
     if(E >= 64)
     {
-        for(int v = v0 + (tid >> 5); v < v1; v += kSortWarps)
-        {
-            if((present[(v - v0) / 32] >> ((v - v0) & 31)) & 1u) continue;
-            float* row = dW + (long long)v * E;
-            if(vec) for(int e = (tid & 31) * 4; e < E; e += 128) st4_stream(row + e, make_float4(0.f, 0.f, 0.f, 0.f));
-            else for(int e = tid & 31; e < E; e += 32) row[e] = 0.f;
-        }
+        for(int r = warp; r < rows; r += kSortWarps)
+            if(!shared.present[r]) zero((r << part_bits) + (int)part + 1);
     }
     else
     {
-        for(long long i = tid; i < (long long)(v1 - v0) * E; i += kSortThreads)
+        for(int i = tid; i < rows * E; i += kSortThreads)
         {
-            const int r = (int)(i / E);
-            if(!((present[r / 32] >> (r & 31)) & 1u)) dW[(long long)v0 * E + i] = 0.f;
+            const int r = i / E;
+            if(!shared.present[r]) dW[((long long)(r << part_bits) + part + 1) * E + i - r * E] = 0.f;
         }
     }
-}
-
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads, 1)
-embedding_sort_kernel(const float* __restrict__ ids, float* __restrict__ dW, uint2* buffer0, uint2* buffer1, int* owner_count,
-                      int tokens, int E, int V, int passes, int digit_bits)
-{
-    extern __shared__ __align__(16) unsigned char bytes[];
-    pdl_launch_dependents();
-    cg::cluster_group cluster = cg::this_cluster();
-    if(blockIdx.x < kSortCtas)
-    {
-        if(blockIdx.x == 0 && threadIdx.x == 0) *owner_count = 0;
-        sort_by_id(*reinterpret_cast<SortShared*>(bytes), ids, buffer0, buffer1, tokens, (unsigned int)V, passes, digit_bits, cluster);
-        return;
-    }
-    const int ctas = gridDim.x - kSortCtas, z = blockIdx.x - kSortCtas;
-    const int rows = (V + ctas - 1) / ctas;
-    const long long v0 = (long long)z * rows;
-    if(v0 < V) zero_absent_rows(reinterpret_cast<unsigned int*>(bytes), ids, dW, tokens, E, (int)v0, (int)(v0 + rows < V ? v0 + rows : V));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -329,12 +379,14 @@ __device__ __forceinline__ void put_row(float* to, typename Piece<VEC>::type sum
     P::store(to, sum);
 }
 
-// A group of `group` threads adds one chunk, group * VEC columns of it.
+constexpr int kLongRun = 4;                       // a run that crosses more chunk edges is long
+
+// A group of `group` threads adds one chunk, group * VEC columns of it.  control = {short runs to join, long ones, sorted positions}.
 template <int VEC, bool TWO>
 __global__ void __launch_bounds__(kReduceThreads)
 embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const float* __restrict__ dY2, float* __restrict__ dW,
-                       float* __restrict__ partial, int* __restrict__ owners, int* owner_count,
-                       int tokens, int E, int V, int chunk, int group, float scale, int accumulate)
+                       float* __restrict__ partial, int* __restrict__ owners, int* control,
+                       int E, int chunk, int chunks, int group, float scale, int accumulate)
 {
     using P = Piece<VEC>;
     using T = typename P::type;
@@ -342,6 +394,7 @@ embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const 
     pdl_wait();
     const int which = threadIdx.x / group;
     const int index = blockIdx.x * (kReduceThreads / group) + which;
+    const int tokens = control[2];
     const int column = (blockIdx.y * group + threadIdx.x % group) * VEC;
     const long long start = (long long)index * chunk;
     if(start >= tokens || column >= E) return;
@@ -353,15 +406,20 @@ embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const 
     T sum = P::zero();
     auto finish = [&](bool ends_here)
     {
-        if(current >= (unsigned int)V) return;         // padding
         if(starts_here && ends_here) put_row<VEC>(dW + (long long)current * E + column, sum, scale, accumulate);
         else
         {
             P::store(partial + ((long long)index * 2 + (starts_here ? 1 : 0)) * E + column, sum);
-            if(starts_here && column == 0) owners[atomicAdd(owner_count, 1)] = index;
+            if(starts_here && column == 0)
+            {
+                // whose partial sums have to be joined: short runs from the front of the list, long ones from its back
+                const long long far = (long long)(index + kLongRun) * chunk;
+                if(far < tokens && sorted[far].x == current) owners[chunks - 1 - atomicAdd(control + 1, 1)] = index;
+                else owners[atomicAdd(control, 1)] = index;
+            }
         }
     };
-    for(int i = (int)start; i < end && current < (unsigned int)V; i += kInFlight)
+    for(int i = (int)start; i < end; i += kInFlight)
     {
         uint2 item[kInFlight];
         T row[kInFlight];
@@ -371,7 +429,7 @@ embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const 
         for(int u = 0; u < kInFlight; u++)
         {
             row[u] = P::zero();
-            if(item[u].x >= (unsigned int)V) continue;
+            if(i + u >= end) continue;
             const long long at = (long long)item[u].y * E + column;
             row[u] = P::load(dY + at);
             if(TWO) row[u] = P::add(row[u], P::load(dY2 + at));
@@ -393,48 +451,50 @@ embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const 
     finish(behind != current);
 }
 
-// A run that starts in one chunk and goes on in the next ones: its last partial of the first chunk, then the first of each
-// following chunk.  Eight warps take every eighth, 32 * VEC columns; their sums are added in order.
+// A run that starts in one chunk and goes on in the next ones: the second partial of its first chunk, then the first of each
+// following one.  A CTA adds 32 * VEC columns of a long run: its eight warps take every eighth part, and their sums are added
+// in order.  A warp adds a short one, four blocks of 32 * VEC columns at a time.
 template <int VEC>
 __global__ void __launch_bounds__(kReduceThreads)
-embedding_join_kernel(const uint2* sorted, const float* partial, const int* owners, const int* owner_count, float* __restrict__ dW,
-                      int tokens, int E, int chunk, float scale, int accumulate)
+embedding_join_kernel(const uint2* sorted, const float* partial, const int* owners, const int* control, float* __restrict__ dW,
+                      int E, int chunk, int chunks, float scale, int accumulate)
 {
     using P = Piece<VEC>;
     using T = typename P::type;
-    __shared__ T warp_sums[kReduceThreads / 32][32];
+    constexpr int kWarps = kReduceThreads / 32;
+    __shared__ T warp_sums[kWarps][32];
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int blocks = (E + 32 * VEC - 1) / (32 * VEC);
-    const long long items = (long long)*owner_count * blocks;
-    for(long long i = blockIdx.x; i < items; i += gridDim.x)
+    const int blocks = (E + 32 * VEC - 1) / (32 * VEC), tokens = control[2];
+    // part 0 of a run is its first chunk's, part j that of the j-th behind it
+    auto part = [&](int index, int j, int column) { return P::load(partial + ((long long)(index + j) * 2 + (j == 0 ? 1 : 0)) * E + column); };
+
+    const long long long_items = (long long)control[1] * blocks;
+    for(long long i = blockIdx.x; i < long_items; i += gridDim.x)
     {
-        const int index = owners[i / blocks];
+        const int index = owners[chunks - 1 - i / blocks];
         const int column = ((int)(i % blocks) * 32 + lane) * VEC;
-        const long long last = (long long)(index + 1) * chunk - 1;       // the chunk is whole: its run goes on behind it
-        const unsigned int v = sorted[last].x;
-        // chunks behind it that begin with the same id
-        int more = 0;
+        const unsigned int v = sorted[(long long)(index + 1) * chunk - 1].x;        // the run goes on behind this chunk
+        int parts = 1;
         while(true)
         {
-            const long long at = (long long)(index + 1 + more + tid) * chunk;
+            // the chunks that begin with the same id lie side by side
+            const long long at = (long long)(index + parts + tid) * chunk;
             const int here = __syncthreads_count(at < tokens && sorted[at].x == v);
-            more += here;
+            parts += here;
             if(here < kReduceThreads) break;
         }
         T sum = P::zero();
         if(column < E)
         {
-            // part 0 is the first chunk's, part j that of the j-th behind it
-            auto part = [&](int j) { return P::load(partial + ((long long)(index + j) * 2 + (j == 0 ? 1 : 0)) * E + column); };
-            for(int j = warp; j <= more; j += 4 * (kReduceThreads / 32))
+            for(int j = warp; j < parts; j += 8 * kWarps)
             {
-                T four[4];
+                T some[8];
 #pragma unroll
-                for(int k = 0; k < 4; k++) four[k] = j + k * (kReduceThreads / 32) <= more ? part(j + k * (kReduceThreads / 32)) : P::zero();
+                for(int k = 0; k < 8; k++) some[k] = j + k * kWarps < parts ? part(index, j + k * kWarps, column) : P::zero();
 #pragma unroll
-                for(int k = 0; k < 4; k++) sum = P::add(sum, four[k]);
+                for(int k = 0; k < 8; k++) sum = P::add(sum, some[k]);
             }
         }
         warp_sums[warp][lane] = sum;
@@ -443,33 +503,65 @@ embedding_join_kernel(const uint2* sorted, const float* partial, const int* owne
         {
             sum = warp_sums[0][lane];
 #pragma unroll
-            for(int w = 1; w < kReduceThreads / 32; w++) sum = P::add(sum, warp_sums[w][lane]);
+            for(int q = 1; q < kWarps; q++) sum = P::add(sum, warp_sums[q][lane]);
             put_row<VEC>(dW + (long long)v * E + column, sum, scale, accumulate);
         }
         __syncthreads();
+    }
+
+    const int short_items = control[0];
+    for(int i = blockIdx.x + warp * gridDim.x; i < short_items; i += gridDim.x * kWarps)
+    {
+        const int index = owners[i];
+        const unsigned int v = sorted[(long long)(index + 1) * chunk - 1].x;
+        const long long at = (long long)(index + 1 + lane) * chunk;
+        const unsigned int other = __ballot_sync(0xffffffffu, !(at < tokens && sorted[at].x == v));
+        const int parts = __ffs(other);                // the chunk itself and those up to the first that begins otherwise: at most kLongRun + 1
+        for(int block = 0; block < blocks; block += 4)
+        {
+            T sum[4];
+#pragma unroll
+            for(int k = 0; k < 4; k++) sum[k] = P::zero();
+#pragma unroll 2
+            for(int j = 0; j < parts; j++)
+            {
+#pragma unroll
+                for(int k = 0; k < 4; k++)
+                {
+                    const int column = ((block + k) * 32 + lane) * VEC;
+                    if(column < E) sum[k] = P::add(sum[k], part(index, j, column));
+                }
+            }
+#pragma unroll
+            for(int k = 0; k < 4; k++)
+            {
+                const int column = ((block + k) * 32 + lane) * VEC;
+                if(column < E) put_row<VEC>(dW + (long long)v * E + column, sum[k], scale, accumulate);
+            }
+        }
     }
 }
 
 // ---------------------------------------------------------------------------------------
 
-constexpr int64_t kFewTokens = 2048;
+// Few positions and a small table: every CTA of the owner kernel reads all ids, and there is one for every 32 rows and 64 columns.
+bool owners_do(int64_t tokens, int64_t E, int64_t V) { return tokens <= 2048 && E * V <= 3 << 20; }
 
 // Positions of a chunk: enough chunks to fill the GPU, few enough that partial sums stay a small share of the traffic.
 int chunk_of(int64_t tokens) { return tokens <= 65536 ? 16 : tokens <= 1048576 ? 32 : 64; }
 
-struct Layout { int64_t buffer0, buffer1, partial, owners, count, words; int chunks; };
+struct Layout { int64_t sorted, partial, owners, control, words; int chunks; };
 
 Layout layout_of(int64_t tokens, int64_t E)
 {
     auto up = [](int64_t words) { return (words + 3) / 4 * 4; };
     Layout l;
     l.chunks = (int)((tokens + chunk_of(tokens) - 1) / chunk_of(tokens));
-    l.buffer0 = 0;
-    l.buffer1 = l.buffer0 + up(2 * tokens);
-    l.partial = l.buffer1 + up(2 * tokens);
+    l.sorted = 0;
+    l.partial = l.sorted + up(2 * tokens);
     l.owners = l.partial + up(2 * (int64_t)l.chunks * E);
-    l.count = l.owners + up(l.chunks);
-    l.words = l.count + 4;
+    l.control = l.owners + up(l.chunks);
+    l.words = l.control + 4;
     return l;
 }
 
@@ -481,12 +573,12 @@ using namespace onn;
 
 static bool sorted_sizes_ok(int64_t B, int64_t S, int64_t E, int64_t V)
 {
-    return B > 0 && S > 0 && E > 0 && V > 0 && E < (1LL << 23) && V < (1LL << 24) && B < (1LL << 31) && S < (1LL << 31) && B * S < (1LL << 31) - 65536;
+    return B > 0 && S > 0 && E > 0 && V > 0 && E < (1LL << 23) && V < (1LL << 23) && B < (1LL << 31) && S < (1LL << 31) && B * S < (1LL << 31) - 65536;
 }
 
 extern "C" size_t onn_embedding_bwd_sorted_workspace_floats(int64_t B, int64_t S, int64_t E, int64_t V)
 {
-    if(!sorted_sizes_ok(B, S, E, V) || B * S <= kFewTokens) return 0;
+    if(!sorted_sizes_ok(B, S, E, V) || owners_do(B * S, E, V)) return 0;
     return (size_t)layout_of(B * S, E).words;
 }
 
@@ -500,9 +592,9 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
     const float scale_value = scale ? sqrtf((float)E) : 1.f;
     const int accumulate = (flags & ONN_ACCUMULATE) ? 1 : 0;
     cudaStream_t s = (cudaStream_t)stream;
-    if(tokens <= kFewTokens)
+    if(owners_do(tokens, E, V))
     {
-        // a CTA for each SM if the table is that tall, but no more rows than fit in shared memory
+        // a few CTAs for each SM if the table is that tall, but no more rows than fit in shared memory
         const int columns = (int)((E + kOwnerColumns - 1) / kOwnerColumns);
         int64_t owned = (V * columns + 2 * kSmCount - 1) / (2 * kSmCount);
         owned = owned < 1 ? 1 : owned > kMaxOwned ? kMaxOwned : owned;
@@ -514,26 +606,20 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
     if(!workspace) return ONN_ERR_WORKSPACE;
     ONN_CHECK_ARG(host_aligned16(workspace));
     const Layout l = layout_of(tokens, E);
-    uint2* buffer0 = reinterpret_cast<uint2*>(workspace + l.buffer0);
-    uint2* buffer1 = reinterpret_cast<uint2*>(workspace + l.buffer1);
+    uint2* sorted = reinterpret_cast<uint2*>(workspace + l.sorted);
     float* partial = workspace + l.partial;
     int* owners = reinterpret_cast<int*>(workspace + l.owners);
-    int* owner_count = reinterpret_cast<int*>(workspace + l.count);
+    int* control = reinterpret_cast<int*>(workspace + l.control);
 
-    int bits = 1;
-    while((V >> bits) != 0) bits++;                    // the largest key is V, for padding
-    const int passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits, digit_bits = (bits + passes - 1) / passes;
     static PerDeviceBytes configured;
-    const int rows_of_zero_cta = (int)((V + kZeroClusters * kSortCtas - 1) / (kZeroClusters * kSortCtas));
-    const size_t bitmap = ((size_t)rows_of_zero_cta + 31) / 32 * 4;
-    const size_t shared = sizeof(SortShared) > bitmap ? sizeof(SortShared) : bitmap;
-    if(!ensure_dynamic_smem(embedding_sort_kernel, configured, shared)) return ONN_ERR_CUDA;
-    embedding_sort_kernel<<<kSortCtas * (accumulate ? 1 : 1 + kZeroClusters), kSortThreads, shared, s>>>(
-        ids, dW, buffer0, buffer1, owner_count, (int)tokens, (int)E, (int)V, passes, digit_bits);
+    if(!ensure_dynamic_smem(embedding_sort_kernel, configured, sizeof(SortShared))) return ONN_ERR_CUDA;
+    int part_bits = 0;
+    while((1 << part_bits) < kMinParts || (V >> part_bits) >= kMaxRows) part_bits++;
+    embedding_sort_kernel<<<1u << part_bits, kSortThreads, sizeof(SortShared), s>>>(
+        ids, sorted, control, dW, (int)tokens, (int)E, (int)V, part_bits, !accumulate);
     count_launch();
     if(launch_status() != ONN_OK) return ONN_ERR_CUDA;
 
-    const uint2* sorted = (passes & 1) ? buffer0 : buffer1;
     const bool vec = (E & 3) == 0 && host_aligned16(dY) && host_aligned16(dY2) && host_aligned16(dW);
     const int pieces = (int)(vec ? E / 4 : E);
     int group = 32;
@@ -542,8 +628,8 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
     const dim3 grid((unsigned)((l.chunks + groups - 1) / groups), (unsigned)((pieces + group - 1) / group));
     auto add = [&](auto kernel)
     {
-        return launch_overlapped(kernel, grid, dim3(kReduceThreads), 0, s, sorted, dY, dY2, dW, partial, owners, owner_count, (int)tokens,
-                                 (int)E, (int)V, chunk, group, scale_value, accumulate);
+        return launch_overlapped(kernel, grid, dim3(kReduceThreads), 0, s, (const uint2*)sorted, dY, dY2, dW, partial, owners, control,
+                                 (int)E, chunk, l.chunks, group, scale_value, accumulate);
     };
     cudaError_t error = vec ? (dY2 ? add(embedding_chunk_kernel<4, true>) : add(embedding_chunk_kernel<4, false>))
                             : (dY2 ? add(embedding_chunk_kernel<1, true>) : add(embedding_chunk_kernel<1, false>));
@@ -551,8 +637,8 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
     if(error != cudaSuccess) return ONN_ERR_CUDA;
     auto join = [&](auto kernel)
     {
-        return launch_overlapped(kernel, dim3(2 * kSmCount), dim3(kReduceThreads), 0, s, sorted, (const float*)partial, (const int*)owners,
-                                 (const int*)owner_count, dW, (int)tokens, (int)E, chunk, scale_value, accumulate);
+        return launch_overlapped(kernel, dim3(4 * kSmCount), dim3(kReduceThreads), 0, s, (const uint2*)sorted, (const float*)partial,
+                                 (const int*)owners, (const int*)control, dW, (int)E, chunk, l.chunks, scale_value, accumulate);
     };
     error = vec ? join(embedding_join_kernel<4>) : join(embedding_join_kernel<1>);
     count_launch();
