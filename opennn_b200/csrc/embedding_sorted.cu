@@ -187,65 +187,60 @@ embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted,
     unsigned short* const list_row = shared.row[warp];
     for(int r = lane; r < rows; r += 32) count[r] = 0;
 
-    // found(n of the lane's first id, the rows of its ids or -1, how many of the warp's lie before the lane's, how many there are)
+    // found(n of the lane's first id, a bit for each of its ids that is one of this CTA's, how many of the warp's lie before the
+    // lane's, how many there are)
     unsigned int lower = 0;
     auto scan = [&](auto found)
     {
         for(long long first = from; first < to; first += kBlock)
         {
             const long long n = first + lane * 16;
-            float id[16];
-#pragma unroll
-            for(int q = 0; q < 4; q++)
+            // 2^23 + id, rounded toward zero, holds trunc(id) in its low bits for 0 <= id < 2^23; everything else (negative, larger,
+            // NaN) comes out far above V - 1 when 2^23 + 1 is taken from the bits
+            unsigned int mine = 0;
+            auto look = [&](float id, int j)
             {
-                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                const long long at = n + q * 4;
-                if(vec && at + 4 <= to) f = __ldg(reinterpret_cast<const float4*>(ids + at));
-                else
+                const unsigned int before = __float_as_uint(__fadd_rz(id, 8388608.f)) - 0x4b000001u;      // id - 1
+                const unsigned int its = before < (unsigned int)(V - 1) ? before & part_mask : 0xffffffffu;
+                lower += its < part;
+                mine |= its == part ? 1u << j : 0u;
+            };
+            if(vec && n + 16 <= to)
+            {
+#pragma unroll
+                for(int q = 0; q < 4; q++)
                 {
-                    if(at < to) f.x = __ldg(ids + at);
-                    if(at + 1 < to) f.y = __ldg(ids + at + 1);
-                    if(at + 2 < to) f.z = __ldg(ids + at + 2);
-                    if(at + 3 < to) f.w = __ldg(ids + at + 3);
+                    const float4 f = __ldg(reinterpret_cast<const float4*>(ids + n) + q);
+                    look(f.x, q * 4); look(f.y, q * 4 + 1); look(f.z, q * 4 + 2); look(f.w, q * 4 + 3);
                 }
-                id[q * 4] = f.x; id[q * 4 + 1] = f.y; id[q * 4 + 2] = f.z; id[q * 4 + 3] = f.w;
             }
-            int row[16], mine = 0;
-#pragma unroll
-            for(int j = 0; j < 16; j++)
+            else
             {
-                // 2^23 + id, rounded toward zero, holds trunc(id) in its low bits for 0 <= id < 2^23; everything else (negative,
-                // larger, NaN) comes out far above V - 1 when 2^23 + 1 is taken from the bits
-                const unsigned int before = __float_as_uint(__fadd_rz(id[j], 8388608.f)) - 0x4b000001u;      // id - 1
-                const bool valid = before < (unsigned int)(V - 1);
-                const unsigned int its = before & part_mask;
-                lower += valid && its < part;
-                row[j] = valid && its == part ? (int)(before >> part_bits) : -1;
-                mine += row[j] >= 0;
+                for(int j = 0; j < 16 && n + j < to; j++) look(__ldg(ids + n + j), j);
             }
             if(!__any_sync(0xffffffffu, mine != 0)) continue;
-            int upto = mine;
+            int upto = __popc(mine);
 #pragma unroll
             for(int offset = 1; offset < 32; offset <<= 1)
             {
                 const int other = __shfl_up_sync(0xffffffffu, upto, offset);
                 if(lane >= offset) upto += other;
             }
-            found((unsigned int)n, row, upto - mine, __shfl_sync(0xffffffffu, upto, 31));
+            found((unsigned int)n, mine, upto - __popc(mine), __shfl_sync(0xffffffffu, upto, 31));
         }
     };
-    auto keep = [&](unsigned int n, const int (&row)[16], int at)
+    auto keep = [&](unsigned int n, unsigned int mine, int at)
     {
-#pragma unroll
-        for(int j = 0; j < 16; j++)
+        for(; mine != 0; mine &= mine - 1, at++)
         {
-            if(row[j] < 0) continue;
-            if(at < kList) { list_position[at] = n + j; list_row[at] = (unsigned short)row[j]; }
-            at++;
+            if(at >= kList) break;
+            const unsigned int position = n + __ffs(mine) - 1;
+            list_position[at] = position;
+            list_row[at] = (unsigned short)((__float_as_uint(__fadd_rz(__ldg(ids + position), 8388608.f)) - 0x4b000001u) >> part_bits);
         }
     };
     int kept = 0;
-    scan([&](unsigned int n, const int (&row)[16], int before, int all) { keep(n, row, kept + before); kept += all; });
+    scan([&](unsigned int n, unsigned int mine, int before, int all) { keep(n, mine, kept + before); kept += all; });
     __syncwarp();
     // the warp's positions in order, 32 at a time: from its list, or from the ids again, 512 of them by way of the list
     auto each = [&](auto act)
@@ -262,9 +257,9 @@ embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted,
         if(kept <= kList) from_list(kept);
         else
         {
-            scan([&](unsigned int n, const int (&row)[16], int before, int all)
+            scan([&](unsigned int n, unsigned int mine, int before, int all)
             {
-                keep(n, row, before);
+                keep(n, mine, before);
                 __syncwarp();
                 from_list(all);
                 __syncwarp();
@@ -385,7 +380,7 @@ constexpr int kLongRun = 4;                       // a run that crosses more chu
 template <int VEC, bool TWO>
 __global__ void __launch_bounds__(kReduceThreads)
 embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const float* __restrict__ dY2, float* __restrict__ dW,
-                       float* __restrict__ partial, int* __restrict__ owners, int* control,
+                       float* __restrict__ partial, int2* __restrict__ owners, int* control,
                        int E, int chunk, int chunks, int group, float scale, int accumulate)
 {
     using P = Piece<VEC>;
@@ -414,8 +409,8 @@ embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const 
             {
                 // whose partial sums have to be joined: short runs from the front of the list, long ones from its back
                 const long long far = (long long)(index + kLongRun) * chunk;
-                if(far < tokens && sorted[far].x == current) owners[chunks - 1 - atomicAdd(control + 1, 1)] = index;
-                else owners[atomicAdd(control, 1)] = index;
+                if(far < tokens && sorted[far].x == current) owners[chunks - 1 - atomicAdd(control + 1, 1)] = make_int2(index, (int)current);
+                else owners[atomicAdd(control, 1)] = make_int2(index, (int)current);
             }
         }
     };
@@ -456,7 +451,7 @@ embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const 
 // in order.  A warp adds a short one, four blocks of 32 * VEC columns at a time.
 template <int VEC>
 __global__ void __launch_bounds__(kReduceThreads)
-embedding_join_kernel(const uint2* sorted, const float* partial, const int* owners, const int* control, float* __restrict__ dW,
+embedding_join_kernel(const uint2* sorted, const float* partial, const int2* owners, const int* control, float* __restrict__ dW,
                       int E, int chunk, int chunks, float scale, int accumulate)
 {
     using P = Piece<VEC>;
@@ -473,9 +468,9 @@ embedding_join_kernel(const uint2* sorted, const float* partial, const int* owne
     const long long long_items = (long long)control[1] * blocks;
     for(long long i = blockIdx.x; i < long_items; i += gridDim.x)
     {
-        const int index = owners[chunks - 1 - i / blocks];
-        const int column = ((int)(i % blocks) * 32 + lane) * VEC;
-        const unsigned int v = sorted[(long long)(index + 1) * chunk - 1].x;        // the run goes on behind this chunk
+        const int2 owner = owners[chunks - 1 - i / blocks];
+        const int index = owner.x, column = ((int)(i % blocks) * 32 + lane) * VEC;
+        const unsigned int v = (unsigned int)owner.y;
         int parts = 1;
         while(true)
         {
@@ -512,8 +507,9 @@ embedding_join_kernel(const uint2* sorted, const float* partial, const int* owne
     const int short_items = control[0];
     for(int i = blockIdx.x + warp * gridDim.x; i < short_items; i += gridDim.x * kWarps)
     {
-        const int index = owners[i];
-        const unsigned int v = sorted[(long long)(index + 1) * chunk - 1].x;
+        const int2 owner = owners[i];
+        const int index = owner.x;
+        const unsigned int v = (unsigned int)owner.y;
         const long long at = (long long)(index + 1 + lane) * chunk;
         const unsigned int other = __ballot_sync(0xffffffffu, !(at < tokens && sorted[at].x == v));
         const int parts = __ffs(other);                // the chunk itself and those up to the first that begins otherwise: at most kLongRun + 1
@@ -548,7 +544,7 @@ embedding_join_kernel(const uint2* sorted, const float* partial, const int* owne
 bool owners_do(int64_t tokens, int64_t E, int64_t V) { return tokens <= 2048 && E * V <= 3 << 20; }
 
 // Positions of a chunk: enough chunks to fill the GPU, few enough that partial sums stay a small share of the traffic.
-int chunk_of(int64_t tokens) { return tokens <= 65536 ? 16 : tokens <= 1048576 ? 32 : 64; }
+int chunk_of(int64_t tokens) { return tokens <= 32768 ? 16 : tokens <= 100000 ? 32 : 64; }
 
 struct Layout { int64_t sorted, partial, owners, control, words; int chunks; };
 
@@ -560,7 +556,7 @@ Layout layout_of(int64_t tokens, int64_t E)
     l.sorted = 0;
     l.partial = l.sorted + up(2 * tokens);
     l.owners = l.partial + up(2 * (int64_t)l.chunks * E);
-    l.control = l.owners + up(l.chunks);
+    l.control = l.owners + up(2 * (int64_t)l.chunks);
     l.words = l.control + 4;
     return l;
 }
@@ -608,7 +604,7 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
     const Layout l = layout_of(tokens, E);
     uint2* sorted = reinterpret_cast<uint2*>(workspace + l.sorted);
     float* partial = workspace + l.partial;
-    int* owners = reinterpret_cast<int*>(workspace + l.owners);
+    int2* owners = reinterpret_cast<int2*>(workspace + l.owners);
     int* control = reinterpret_cast<int*>(workspace + l.control);
 
     static PerDeviceBytes configured;
@@ -638,7 +634,7 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
     auto join = [&](auto kernel)
     {
         return launch_overlapped(kernel, dim3(4 * kSmCount), dim3(kReduceThreads), 0, s, (const uint2*)sorted, (const float*)partial,
-                                 (const int*)owners, (const int*)control, dW, (int)E, chunk, l.chunks, scale_value, accumulate);
+                                 (const int2*)owners, (const int*)control, dW, (int)E, chunk, l.chunks, scale_value, accumulate);
     };
     error = vec ? join(embedding_join_kernel<4>) : join(embedding_join_kernel<1>);
     count_launch();
