@@ -187,12 +187,19 @@ def _i32(t, shape, what):
     return t.data_ptr()
 
 
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream      # the handle alone: a twentieth of the time
+except ImportError:
+    def _raw_stream(device):
+        return torch.cuda.current_stream(device).cuda_stream
+
+
 def _current_stream(t):
     """The current stream, which has to be one of the device that holds t."""
-    stream = torch.cuda.current_stream()
-    if t.get_device() != stream.device_index:
-        raise OnnError(f"the tensors are on cuda:{t.get_device()}, the current device is cuda:{stream.device_index}")
-    return stream.cuda_stream
+    device = torch.cuda.current_device()
+    if t.get_device() != device:
+        raise OnnError(f"the tensors are on cuda:{t.get_device()}, the current device is cuda:{device}")
+    return _raw_stream(device)
 
 
 def embedding_bwd_sorted(ids, dY, V, scale=True, dY2=None, dW=None, accumulate=False):

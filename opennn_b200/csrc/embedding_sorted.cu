@@ -31,7 +31,7 @@ constexpr int kOwnerWarps = kOwnerThreads / 32;
 constexpr int kTile = 1024;                       // ids looked at together
 constexpr int kOwnerColumns = 64;
 constexpr int kOwnerGroups = kOwnerThreads / kOwnerColumns;
-constexpr int kOwnerInFlight = 8;                 // gradient elements a thread has under way
+constexpr int kOwnerInFlight = 16;                // gradient elements a thread has under way
 constexpr int kMaxOwned = 32;                     // rows of a CTA, summed in shared memory
 
 // CTA (x, y) owns `owned` consecutive rows of the table, 64 columns of them.  It walks over all ids in order and keeps those that

@@ -192,6 +192,11 @@ __device__ __forceinline__ long long row_token(const float* tokens, long long ro
 template <typename... KernelArgs, typename... Args>
 inline cudaError_t launch_clusters(void (*kernel)(KernelArgs...), unsigned int grid, int threads, int ctas, size_t dynamic_bytes, bool overlapped, cudaStream_t stream, Args&&... args)
 {
+    if(ctas == 1 && !overlapped)
+    {
+        kernel<<<grid, threads, dynamic_bytes, stream>>>(std::forward<Args>(args)...);      // half the host's time of the launch below
+        return cudaGetLastError();
+    }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);

@@ -18,8 +18,6 @@ namespace onn
 namespace
 {
 
-constexpr int kThreads = 256;                     // of the backward pass
-constexpr int kUnroll = 8;                        // 16-byte vectors a thread has in flight
 
 // Running statistics of a set of logits, in base 2 and relative to the largest logit m seen: with c = log2(e) / T,
 // a = c max(m, -kHuge) and d = c x - a in one rounding,  s = sum 2^d  and  w = sum 2^d d.  Every set with the
@@ -568,9 +566,9 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     if(ctas > 1) cluster.sync();
 }
 
-// One CTA per piece of a row: the row's scalars, then load, compute, store.
-template <int DTYPE>
-__global__ void __launch_bounds__(kThreads)
+// One CTA per piece of a row: the row's scalars, then batches of vectors: load, compute, store.
+template <int DTYPE, bool ENTROPY, int T, int N>
+__global__ void __launch_bounds__(T, 1024 / T)
 token_logprobs_bwd_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, const float* __restrict__ tokens,
                           const float* __restrict__ lse, const float* __restrict__ entropy,
                           const float* __restrict__ d_logprobs, const float* __restrict__ d_entropy,
@@ -580,54 +578,84 @@ token_logprobs_bwd_kernel(const typename Logit<DTYPE>::type* logits, long long p
     constexpr int VE = L::VE;
     const long long row = blockIdx.y;
     const int tid = threadIdx.x;
-    bool active;
-    const long long token = row_token(tokens, row, V, &active);
     const typename L::type* x = logits + row * pitch;
     typename L::type* dx = dlogits + row * d_pitch;
     const RowCut cut = cut_row<DTYPE>(dx, V);
-    const bool together = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
-
-    const float g = active ? d_logprobs[row] * inverse_temperature : 0.f;
-    const float h = active && d_entropy ? d_entropy[row] * inverse_temperature : 0.f;
-    const float H = h != 0.f ? entropy[row] : 0.f;
-    float row_lse = active ? lse[row] : 0.f;
-    if(row_lse == -INFINITY) row_lse = 0.f;            // a row without a finite logit: every p is 0
-
-    auto one = [&](float value, long long index)
+    const int after = cut.head + cut.vectors * VE;
+    const int end_index = blockIdx.x != 0 ? -1 : tid < cut.head ? tid : tid < cut.head + cut.tail ? after + tid - cut.head : -1;
+    bool active;
+    const long long token = row_token(tokens, row, V, &active);
+    if(!active)
     {
-        if(!active) return 0.f;
-        const float log_p = fmaf(value, inverse_temperature, -row_lse);
-        const float p = exp2_approx(log_p * kLog2E);
-        float r = -g * p;
-        if(h != 0.f) r = fmaf(-h * p, fmaxf(log_p, kNothing) + H, r);
-        if(index == token) r += g;
-        return r;
+        for(int i = blockIdx.x * T + tid; i < cut.vectors; i += gridDim.x * T)
+            *reinterpret_cast<uint4*>(dx + cut.head + i * VE) = make_uint4(0u, 0u, 0u, 0u);
+        if(end_index >= 0) L::put(dx + end_index, 0.f);
+        return;
+    }
+    const float g = d_logprobs[row] * inverse_temperature;
+    const float h = ENTROPY ? d_entropy[row] * inverse_temperature : 0.f;
+    const float H = ENTROPY ? entropy[row] : 0.f;
+    float row_lse = lse[row];
+    if(row_lse == -INFINITY) row_lse = 0.f;            // a row without a finite logit: every p is 0
+    const float2 minus_lse = make_float2(-row_lse, -row_lse), it2 = make_float2(inverse_temperature, inverse_temperature);
+    const float2 log2e2 = make_float2(kLog2E, kLog2E), minus_g = make_float2(-g, -g), minus_h = make_float2(-h, -h), H2 = make_float2(H, H);
+    auto two = [&](float2 value)
+    {
+        const float2 log_p = fma2(value, it2, minus_lse);
+        const float2 d = mul2(log_p, log2e2);
+        const float2 p = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+        if(!ENTROPY) return mul2(minus_g, p);
+        const float2 inner = add2(make_float2(fmaxf(log_p.x, kNothing), fmaxf(log_p.y, kNothing)), H2);
+        return mul2(fma2(minus_h, inner, minus_g), p);
     };
 
-    const int after = cut.head + cut.vectors * VE;
-    if(blockIdx.x == 0 && tid < cut.head + cut.tail)
+    if(end_index >= 0)
     {
-        const int i = tid < cut.head ? tid : after + tid - cut.head;
-        L::put(dx + i, one(active ? L::get(x + i) : 0.f, i));
+        const float value = L::get(x + end_index);
+        L::put(dx + end_index, two(make_float2(value, value)).x + (end_index == (int)token ? g : 0.f));
     }
-    for(int i = blockIdx.x * kThreads + tid; i < cut.vectors; i += gridDim.x * kThreads)
+    const bool together = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+    const int token_vector = (int)token >= cut.head && (int)token < after ? ((int)token - cut.head) / VE : -1;
+    const int token_place = ((int)token - cut.head) % VE;
+    for(int first = blockIdx.x * (T * N) + tid; first < cut.vectors; first += gridDim.x * (T * N))
     {
-        const int index = cut.head + i * VE;
-        float f[VE];
-        if(!active)
+        uint4 v[N];
+#pragma unroll
+        for(int u = 0; u < N; u++)
         {
+            const int i = first + u * T;
+            if(i >= cut.vectors) continue;
+            const typename L::type* at = x + cut.head + i * VE;
+            if(together) v[u] = __ldcs(reinterpret_cast<const uint4*>(at));
+            else
+            {
+                float f[VE];
 #pragma unroll
-            for(int e = 0; e < VE; e++) f[e] = 0.f;
+                for(int e = 0; e < VE; e++) f[e] = L::get(at + e);
+                v[u] = L::pack(f);                     // exact: the values come from this type
+            }
         }
-        else if(together) L::unpack(*reinterpret_cast<const uint4*>(x + index), f);
-        else
+#pragma unroll
+        for(int u = 0; u < N; u++)
         {
+            const int i = first + u * T;
+            if(i >= cut.vectors) continue;
+            float f[VE];
+            L::unpack(v[u], f);
 #pragma unroll
-            for(int e = 0; e < VE; e++) f[e] = L::get(x + index + e);
+            for(int e = 0; e < VE; e += 2)
+            {
+                const float2 r = two(make_float2(f[e], f[e + 1]));
+                f[e] = r.x;
+                f[e + 1] = r.y;
+            }
+            if(i == token_vector)
+            {
+#pragma unroll
+                for(int e = 0; e < VE; e++) f[e] += e == token_place ? g : 0.f;
+            }
+            *reinterpret_cast<uint4*>(dx + cut.head + i * VE) = L::pack(f);
         }
-#pragma unroll
-        for(int e = 0; e < VE; e++) f[e] = one(f[e], index + e);
-        *reinterpret_cast<uint4*>(dx + index) = L::pack(f);
     }
 }
 
@@ -675,13 +703,19 @@ int launch_bwd(const void* logits, int64_t pitch, const float* tokens, const flo
                float inverse_temperature, cudaStream_t stream)
 {
     using L = Logit<DTYPE>;
-    const int pieces = (int)((V / L::VE + kThreads * kUnroll - 1) / (kThreads * kUnroll));
+    // small CTAs for short rows (16384 x 1000 bf16: 14.7 us, with 256 threads 35), pieces of eight vectors per thread
+    const int64_t vectors = V / L::VE;
+    const int T = vectors <= 256 ? 64 : vectors <= 2048 ? 128 : 256;
+    const int pieces = (int)((vectors + T * 8 - 1) / (T * 8));
+    const auto kernel = T == 64 ? (d_entropy ? token_logprobs_bwd_kernel<DTYPE, true, 64, 4> : token_logprobs_bwd_kernel<DTYPE, false, 64, 4>)
+                      : T == 128 ? (d_entropy ? token_logprobs_bwd_kernel<DTYPE, true, 128, 4> : token_logprobs_bwd_kernel<DTYPE, false, 128, 4>)
+                                 : (d_entropy ? token_logprobs_bwd_kernel<DTYPE, true, 256, 4> : token_logprobs_bwd_kernel<DTYPE, false, 256, 4>);
     // the second grid dimension holds at most 65535 rows
     for(int64_t first = 0; first < rows; first += 65535)
     {
         const int64_t n = rows - first < 65535 ? rows - first : 65535;
-        token_logprobs_bwd_kernel<DTYPE><<<dim3(pieces > 0 ? pieces : 1, (unsigned)n), kThreads, 0, stream>>>(
-            static_cast<const typename L::type*>(logits) + first * pitch, pitch, tokens ? tokens + first : nullptr, lse + first,
+        kernel<<<dim3(pieces > 0 ? pieces : 1, (unsigned)n), T, 0, stream>>>(
+            static_cast<const typename L::type*>(logits) + first * pitch, pitch, tokens + first, lse + first,
             entropy ? entropy + first : nullptr, d_logprobs + first, d_entropy ? d_entropy + first : nullptr,
             static_cast<typename L::type*>(dlogits) + first * d_pitch, d_pitch, (int)V, inverse_temperature);
         count_launch();
