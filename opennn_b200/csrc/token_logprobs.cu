@@ -179,6 +179,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
 {
     using L = Logit<DTYPE>;
     constexpr int VE = L::VE, kWarps = T / 32;
+    constexpr bool kAhead = DTYPE != ONN_F32 && TOP;
     __shared__ Shared<TOP, T> shared;
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -259,16 +260,23 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             best = fmaxf(best, value);
         }
     };
-    auto take = [&](const int batch, auto whole)
+    const int whole = (end - begin) / (T * N), batches = (each + N - 1) / N;
+    auto load = [&](uint4 (&v)[N], const int batch)
     {
-        const int first = begin + batch * (T * N);
-        uint4 v[N];
-#pragma unroll
-        for(int u = 0; u < N; u++)
+        const int first = begin + batch * (T * N) + tid;
+        if(batch < whole)
         {
-            const int i = first + u * T + tid;
-            v[u] = whole.value || i < end ? __ldg(body + i) : L::lowest();
+#pragma unroll
+            for(int u = 0; u < N; u++) v[u] = __ldg(body + first + u * T);
         }
+        else
+        {
+#pragma unroll
+            for(int u = 0; u < N; u++) v[u] = first + u * T < end ? __ldg(body + first + u * T) : L::lowest();
+        }
+    };
+    auto take = [&](const uint4 (&v)[N], const int batch)
+    {
         float vector_max[N];
         float m = -INFINITY;
 #pragma unroll
@@ -294,11 +302,27 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         }
         add_vectors<DTYPE, N>(r, v, fmaxf(r.m, m), c);
     };
+    if constexpr(kAhead)
     {
-        const int whole = (end - begin) / (T * N), batches = (each + N - 1) / N;
-        int batch = 0;
-        for(; batch < whole; batch++) take(batch, std::true_type{});
-        for(; batch < batches; batch++) take(batch, std::false_type{});
+        // a batch is on its way while the one before it is worked on
+        uint4 v[N], next[N];
+        load(next, 0);
+        for(int batch = 0; batch < batches; batch++)
+        {
+#pragma unroll
+            for(int u = 0; u < N; u++) v[u] = next[u];
+            if(batch + 1 < batches) load(next, batch + 1);
+            take(v, batch);
+        }
+    }
+    else
+    {
+        for(int batch = 0; batch < batches; batch++)
+        {
+            uint4 v[N];
+            load(v, batch);
+            take(v, batch);
+        }
     }
 
     // every warp's part to every CTA of the cluster
