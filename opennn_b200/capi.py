@@ -211,9 +211,10 @@ def embedding_bwd_sorted(ids, dY, V, scale=True, dY2=None, dW=None, accumulate=F
     L = lib()
     n = B * S
     stream = _current_stream(dY)
-    workspace = _empty(L.onn_embedding_bwd_sorted_workspace_floats(B, S, E, V))
+    floats = L.onn_embedding_bwd_sorted_workspace_floats(B, S, E, V)
+    workspace = _empty(floats) if floats else None
     check(L.onn_embedding_bwd_sorted(_f32(ids, n, "ids"), _f32(dY, n * E, "dY"), _f32(dY2, n * E, "dY2"), _f32(dW, V * E, "dW"),
-                                     B, S, E, V, int(scale), workspace.data_ptr(), ACCUMULATE if accumulate else 0, stream),
+                                     B, S, E, V, int(scale), _f32(workspace, floats, "workspace"), ACCUMULATE if accumulate else 0, stream),
           "onn_embedding_bwd_sorted")
     return dW
 

@@ -189,8 +189,9 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         if(tid == 0) shared.candidate_count = 0;
         for(int i = tid; i <= kBuckets; i += T) shared.bucket[i] = 0;
     }
-    // all CTAs of a cluster must be running before one writes into another
-    if(ctas > 1) cluster.sync();
+    // all CTAs of a cluster must be running before one writes into another: waited for under the first row's loads
+    bool met = ctas == 1;
+    if(!met) asm volatile("barrier.cluster.arrive;" ::: "memory");
 
     int flip = 0;
     const long long step = gridDim.x / ctas;
@@ -342,6 +343,8 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     }
     else
     {
+        if(!met) asm volatile("barrier.cluster.wait;" ::: "memory");
+        met = true;
         if(lane < ctas) cluster.map_shared_rank(&shared, lane)->parts[flip][rank * kWarps + warp] = part;
         cluster.sync();
     }
@@ -381,16 +384,9 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         float bound;
         if(wanted == 1 && parts >= 2 * top)
         {
-            // more warps than places: the bound is the top-th largest of their maxima
-            float found = -INFINITY;
-            for(int i = lane; i < parts; i += 32)
-            {
-                const float mine = row_parts[i].m;
-                int larger = 0;
-                for(int j = 0; j < parts; j++) larger += row_parts[j].m > mine || (row_parts[j].m == mine && j < i);
-                if(larger == top - 1) found = mine;
-            }
-            bound = warp_max(found);
+            // more warps than places: the bound is the top-th largest of their maxima, at most two of them a lane's
+            const float a = lane < parts ? row_parts[lane].m : -INFINITY, b = lane + 32 < parts ? row_parts[lane + 32].m : -INFINITY;
+            bound = warp_reached_by(fmaxf(a, b), fminf(a, b), top);
         }
         else
         {
@@ -586,8 +582,8 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         if(tid == 0) shared.candidate_count = 0;
     }
     }
-    // no CTA of a cluster ends while another may still write into it
-    if(ctas > 1) cluster.sync();
+    // whatever one CTA of a cluster writes into another comes before the last barrier of the row
+    if(!met) asm volatile("barrier.cluster.wait;" ::: "memory");
 }
 
 // One CTA per piece of a row: the row's scalars, then batches of vectors: load, compute, store.
