@@ -7,10 +7,11 @@
 //      frequent together): it reads all ids, keeps the positions of its own, counts those of the CTAs before it, which
 //      tells where its part of the sorted list begins, and sorts what it has kept.  No CTA needs another's result, so one
 //      launch does it: 6.5 us for 16384 positions (a radix sort by one cluster, or in launches of counts and places: 14 to
-//      20).  The same CTA writes the zeros of its rows that do not occur;
+//      20);
 //   2  the sorted positions are cut into equal chunks, whatever their ids, so that a frequent token is spread over many
 //      CTAs; a group of threads adds the rows of a chunk, and writes the table row of each run of equal ids that lies inside it.
-//      Runs that cross the edge of a chunk leave a partial sum;
+//      Runs that cross the edge of a chunk leave a partial sum.  Other CTAs of the same launch write the zeros of the
+//      table rows that do not occur;
 //   3  the partial sums of each run that crosses an edge are added in order.
 // Few positions take one launch instead: every CTA owns some rows of the table and looks for their ids itself.
 #include "common.cuh"
@@ -132,7 +133,7 @@ embedding_owner_kernel(const float* __restrict__ ids, const float* __restrict__ 
 }
 
 // ---------------------------------------------------------------------------------------
-// 1: sort, and the zeros
+// 1: sort
 // ---------------------------------------------------------------------------------------
 
 constexpr int kSortThreads = 1024;
@@ -147,9 +148,9 @@ struct SortShared
     unsigned int count[kSortWarps][kMaxRows];     // of each warp: how often a row occurs; then where its next position goes
     unsigned int position[kSortWarps][kList];
     unsigned short row[kSortWarps][kList];
+    unsigned short place[kSortWarps][kList];      // among the warp's positions of the same row
     unsigned int warp_sum[kSortWarps];
     unsigned int warp_lower[kSortWarps];
-    unsigned char present[kMaxRows];
 };
 
 // The lanes of the warp whose row is this lane's: one vote per bit.
@@ -166,10 +167,10 @@ __device__ __forceinline__ unsigned int lanes_with(unsigned int row, bool there)
 }
 
 // CTA c has the rows v of the table with (v - 1) % parts = c, parts = 1 << part_bits; its row r is v = (r << part_bits) + c + 1.
-// (The last CTA has row 0 as well, which no position has.)  Warp w looks at the w-th of 32 equal stretches of the ids.
+// Warp w looks at the w-th of 32 equal stretches of the ids.  present[v] says whether v occurs.
 __global__ void __launch_bounds__(kSortThreads, 1)
-embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted, int* __restrict__ control, float* __restrict__ dW,
-                      int tokens, int E, int V, int part_bits, int write_zeros)
+embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted, int* __restrict__ control,
+                      unsigned char* __restrict__ present, int tokens, int V, int part_bits)
 {
     extern __shared__ __align__(16) unsigned char bytes[];
     SortShared& shared = *reinterpret_cast<SortShared*>(bytes);
@@ -185,6 +186,7 @@ embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted,
     unsigned int* const count = shared.count[warp];
     unsigned int* const list_position = shared.position[warp];
     unsigned short* const list_row = shared.row[warp];
+    unsigned short* const list_place = shared.place[warp];
     for(int r = lane; r < rows; r += 32) count[r] = 0;
 
     // found(n of the lane's first id, a bit for each of its ids that is one of this CTA's, how many of the warp's lie before the
@@ -242,19 +244,20 @@ embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted,
     int kept = 0;
     scan([&](unsigned int n, unsigned int mine, int before, int all) { keep(n, mine, kept + before); kept += all; });
     __syncwarp();
-    // the warp's positions in order, 32 at a time: from its list, or from the ids again, 512 of them by way of the list
+    // act(whether there is one, its row, position, index on the list) for the warp's positions in order, 32 at a time: from its
+    // list, or, where it is too short, from the ids again, 512 of them by way of the list
+    const bool listed = kept <= kList;
     auto each = [&](auto act)
     {
         auto from_list = [&](int n)
         {
-            for(int i = 0; i < n; i += 32)
+            for(int i = lane; i - lane < n; i += 32)
             {
-                const bool there = i + lane < n;
-                const unsigned int row = there ? list_row[i + lane] : 0u;
-                act(there, row, there ? list_position[i + lane] : 0u, lanes_with(row, there));
+                const bool there = i < n;
+                act(there, there ? list_row[i] : 0u, there ? list_position[i] : 0u, i);
             }
         };
-        if(kept <= kList) from_list(kept);
+        if(listed) from_list(kept);
         else
         {
             scan([&](unsigned int n, unsigned int mine, int before, int all)
@@ -268,10 +271,20 @@ embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted,
     };
     const unsigned int lower_of_warp = __reduce_add_sync(0xffffffffu, lower);
     if(lane == 0) shared.warp_lower[warp] = lower_of_warp;
-    each([&](bool there, unsigned int row, unsigned int, unsigned int same)
+    // the place of a position among the warp's of its row, which count[row] counts up
+    auto next_place = [&](bool there, unsigned int row)
     {
+        const unsigned int same = lanes_with(row, there);
+        const unsigned int place = there ? count[row] + __popc(same & below) : 0u;
+        __syncwarp();
         if(there && (same & below) == 0) count[row] += __popc(same);
         __syncwarp();
+        return place;
+    };
+    each([&](bool there, unsigned int row, unsigned int, int i)
+    {
+        const unsigned int place = next_place(there, row);
+        if(listed && there) list_place[i] = (unsigned short)place;
     });
     __syncthreads();
 
@@ -281,8 +294,9 @@ embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted,
     {
 #pragma unroll 8
         for(int w = 0; w < kSortWarps; w++) all += shared.count[w][tid];
-        shared.present[tid] = all != 0;
+        present[(tid << part_bits) + part + 1] = all != 0;
     }
+    if(tid == 0 && part == 0) present[0] = 0;
     unsigned int upto = all;
 #pragma unroll
     for(int offset = 1; offset < 32; offset <<= 1)
@@ -305,37 +319,11 @@ embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted,
         }
     }
     __syncthreads();
-    each([&](bool there, unsigned int row, unsigned int position, unsigned int same)
+    each([&](bool there, unsigned int row, unsigned int position, int i)
     {
-        const unsigned int at = there ? count[row] + __popc(same & below) : 0u;
-        __syncwarp();
+        const unsigned int at = listed ? there ? count[row] + list_place[i] : 0u : next_place(there, row);
         if(there) sorted[at] = make_uint2((row << part_bits) + part + 1u, position);
-        if(there && (same & below) == 0) count[row] += __popc(same);
-        __syncwarp();
     });
-
-    if(!write_zeros) return;
-    const bool vec_rows = (E & 3) == 0 && aligned16(dW);
-    auto zero = [&](int v)
-    {
-        float* to_row = dW + (long long)v * E;
-        if(vec_rows) for(int e = lane * 4; e < E; e += 128) st4(to_row + e, make_float4(0.f, 0.f, 0.f, 0.f));
-        else for(int e = lane; e < E; e += 32) to_row[e] = 0.f;
-    };
-    if(part == part_mask && warp == 0) zero(0);
-    if(E >= 64)
-    {
-        for(int r = warp; r < rows; r += kSortWarps)
-            if(!shared.present[r]) zero((r << part_bits) + (int)part + 1);
-    }
-    else
-    {
-        for(int i = tid; i < rows * E; i += kSortThreads)
-        {
-            const int r = i / E;
-            if(!shared.present[r]) dW[((long long)(r << part_bits) + part + 1) * E + i - r * E] = 0.f;
-        }
-    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -376,27 +364,62 @@ __device__ __forceinline__ void put_row(float* to, typename Piece<VEC>::type sum
 
 constexpr int kLongRun = 4;                       // a run that crosses more chunk edges is long
 
+constexpr int kMaxChunk = 64;
+constexpr int kZeroRows = 32;                     // table rows of a CTA that writes zeros
+
+template <int VEC>
+__device__ void zero_absent_rows(const unsigned char* present, float* __restrict__ dW, int E, int V, long long v0)
+{
+    using P = Piece<VEC>;
+    const int pieces = E / VEC, tid = threadIdx.x;
+    const int rows = (int)(V - v0 < kZeroRows ? V - v0 : kZeroRows);
+    if(pieces >= 32)
+    {
+        for(int r = tid >> 5; r < rows; r += kReduceThreads / 32)
+        {
+            if(present[v0 + r]) continue;
+            for(int e = tid & 31; e < pieces; e += 32) P::store(dW + (v0 + r) * E + e * VEC, P::zero());
+        }
+    }
+    else
+    {
+        for(int i = tid; i < rows * pieces; i += kReduceThreads)
+            if(!present[v0 + i / pieces]) P::store(dW + v0 * E + (long long)i * VEC, P::zero());
+    }
+}
+
 // A group of `group` threads adds one chunk, group * VEC columns of it.  control = {short runs to join, long ones, sorted positions}.
+// CTAs behind the first `chunk_ctas` write zeros.
 template <int VEC, bool TWO>
-__global__ void __launch_bounds__(kReduceThreads)
-embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const float* __restrict__ dY2, float* __restrict__ dW,
-                       float* __restrict__ partial, int2* __restrict__ owners, int* control,
-                       int E, int chunk, int chunks, int group, float scale, int accumulate)
+__global__ void __launch_bounds__(kReduceThreads, TWO ? 2 : 3)
+embedding_chunk_kernel(const uint2* sorted, const unsigned char* present, const float* __restrict__ dY, const float* __restrict__ dY2,
+                       float* __restrict__ dW, float* __restrict__ partial, int2* __restrict__ owners, int* control,
+                       int E, int V, int chunk, int chunks, int chunk_ctas, int group, float scale, int accumulate)
 {
     using P = Piece<VEC>;
     using T = typename P::type;
+    __shared__ uint2 items[kReduceThreads / 32][kMaxChunk];
     pdl_launch_dependents();
     pdl_wait();
+    if((int)blockIdx.x >= chunk_ctas)
+    {
+        if(blockIdx.y == 0) zero_absent_rows<VEC>(present, dW, E, V, (long long)(blockIdx.x - chunk_ctas) * kZeroRows);
+        return;
+    }
     const int which = threadIdx.x / group;
     const int index = blockIdx.x * (kReduceThreads / group) + which;
     const int tokens = control[2];
     const int column = (blockIdx.y * group + threadIdx.x % group) * VEC;
     const long long start = (long long)index * chunk;
-    if(start >= tokens || column >= E) return;
-    const int end = (int)(start + chunk < tokens ? start + chunk : tokens);
+    const int length = (int)(start < tokens ? (tokens - start < chunk ? tokens - start : chunk) : 0);
+    for(int i = threadIdx.x % group; i < length; i += group) items[which][i] = sorted[start + i];
+    __syncthreads();
+    if(length == 0 || column >= E) return;
+    const uint2* const item = items[which];
+    const long long end = start + length;
     const unsigned int before = start > 0 ? sorted[start - 1].x : 0xffffffffu, behind = end < tokens ? sorted[end].x : 0xffffffffu;
 
-    unsigned int current = sorted[start].x;
+    unsigned int current = item[0].x;
     bool starts_here = before != current;
     T sum = P::zero();
     auto finish = [&](bool ends_here)
@@ -414,33 +437,31 @@ embedding_chunk_kernel(const uint2* sorted, const float* __restrict__ dY, const 
             }
         }
     };
-    for(int i = (int)start; i < end; i += kInFlight)
+    for(int i = 0; i < length; i += kInFlight)
     {
-        uint2 item[kInFlight];
-        T row[kInFlight];
-#pragma unroll
-        for(int u = 0; u < kInFlight; u++) item[u] = i + u < end ? sorted[i + u] : make_uint2(0xffffffffu, 0u);
+        T row[kInFlight], other[kInFlight];
 #pragma unroll
         for(int u = 0; u < kInFlight; u++)
         {
-            row[u] = P::zero();
-            if(i + u >= end) continue;
-            const long long at = (long long)item[u].y * E + column;
+            row[u] = other[u] = P::zero();
+            if(i + u >= length) continue;
+            const long long at = (long long)item[i + u].y * E + column;
             row[u] = P::load(dY + at);
-            if(TWO) row[u] = P::add(row[u], P::load(dY2 + at));
+            if(TWO) other[u] = P::load(dY2 + at);
         }
 #pragma unroll
         for(int u = 0; u < kInFlight; u++)
         {
-            if(i + u >= end) break;
-            if(item[u].x != current)
+            if(i + u >= length) break;
+            const unsigned int v = item[i + u].x;
+            if(v != current)
             {
                 finish(true);
-                current = item[u].x;
+                current = v;
                 starts_here = true;
                 sum = P::zero();
             }
-            sum = P::add(sum, row[u]);
+            sum = P::add(sum, TWO ? P::add(row[u], other[u]) : row[u]);
         }
     }
     finish(behind != current);
@@ -546,9 +567,9 @@ bool owners_do(int64_t tokens, int64_t E, int64_t V) { return tokens <= 2048 && 
 // Positions of a chunk: enough chunks to fill the GPU, few enough that partial sums stay a small share of the traffic.
 int chunk_of(int64_t tokens) { return tokens <= 32768 ? 16 : tokens <= 100000 ? 32 : 64; }
 
-struct Layout { int64_t sorted, partial, owners, control, words; int chunks; };
+struct Layout { int64_t sorted, partial, owners, control, present, words; int chunks; };
 
-Layout layout_of(int64_t tokens, int64_t E)
+Layout layout_of(int64_t tokens, int64_t E, int64_t V)
 {
     auto up = [](int64_t words) { return (words + 3) / 4 * 4; };
     Layout l;
@@ -557,7 +578,8 @@ Layout layout_of(int64_t tokens, int64_t E)
     l.partial = l.sorted + up(2 * tokens);
     l.owners = l.partial + up(2 * (int64_t)l.chunks * E);
     l.control = l.owners + up(2 * (int64_t)l.chunks);
-    l.words = l.control + 4;
+    l.present = l.control + 4;
+    l.words = l.present + up((V + 3) / 4);
     return l;
 }
 
@@ -575,7 +597,7 @@ static bool sorted_sizes_ok(int64_t B, int64_t S, int64_t E, int64_t V)
 extern "C" size_t onn_embedding_bwd_sorted_workspace_floats(int64_t B, int64_t S, int64_t E, int64_t V)
 {
     if(!sorted_sizes_ok(B, S, E, V) || owners_do(B * S, E, V)) return 0;
-    return (size_t)layout_of(B * S, E).words;
+    return (size_t)layout_of(B * S, E, V).words;
 }
 
 extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const float* dY2, float* dW,
@@ -601,18 +623,19 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
     }
     if(!workspace) return ONN_ERR_WORKSPACE;
     ONN_CHECK_ARG(host_aligned16(workspace));
-    const Layout l = layout_of(tokens, E);
+    const Layout l = layout_of(tokens, E, V);
     uint2* sorted = reinterpret_cast<uint2*>(workspace + l.sorted);
     float* partial = workspace + l.partial;
     int2* owners = reinterpret_cast<int2*>(workspace + l.owners);
     int* control = reinterpret_cast<int*>(workspace + l.control);
+    unsigned char* present = reinterpret_cast<unsigned char*>(workspace + l.present);
 
     static PerDeviceBytes configured;
     if(!ensure_dynamic_smem(embedding_sort_kernel, configured, sizeof(SortShared))) return ONN_ERR_CUDA;
     int part_bits = 0;
     while((1 << part_bits) < kMinParts || (V >> part_bits) >= kMaxRows) part_bits++;
     embedding_sort_kernel<<<1u << part_bits, kSortThreads, sizeof(SortShared), s>>>(
-        ids, sorted, control, dW, (int)tokens, (int)E, (int)V, part_bits, !accumulate);
+        ids, sorted, control, present, (int)tokens, (int)V, part_bits);
     count_launch();
     if(launch_status() != ONN_OK) return ONN_ERR_CUDA;
 
@@ -621,11 +644,13 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
     int group = 32;
     while(group < kReduceThreads && group < pieces) group *= 2;
     const int chunk = chunk_of(tokens), groups = kReduceThreads / group;
-    const dim3 grid((unsigned)((l.chunks + groups - 1) / groups), (unsigned)((pieces + group - 1) / group));
+    const int chunk_ctas = (l.chunks + groups - 1) / groups, zero_ctas = accumulate ? 0 : (int)((V + kZeroRows - 1) / kZeroRows);
+    const dim3 grid((unsigned)(chunk_ctas + zero_ctas), (unsigned)((pieces + group - 1) / group));
     auto add = [&](auto kernel)
     {
-        return launch_overlapped(kernel, grid, dim3(kReduceThreads), 0, s, (const uint2*)sorted, dY, dY2, dW, partial, owners, control,
-                                 (int)E, chunk, l.chunks, group, scale_value, accumulate);
+        return launch_overlapped(kernel, grid, dim3(kReduceThreads), 0, s, (const uint2*)sorted,
+                                 (const unsigned char*)present, dY, dY2, dW, partial, owners, control, (int)E, (int)V, chunk, l.chunks,
+                                 chunk_ctas, group, scale_value, accumulate);
     };
     cudaError_t error = vec ? (dY2 ? add(embedding_chunk_kernel<4, true>) : add(embedding_chunk_kernel<4, false>))
                             : (dY2 ? add(embedding_chunk_kernel<1, true>) : add(embedding_chunk_kernel<1, false>));
