@@ -331,8 +331,6 @@ embedding_sort_kernel(const float* __restrict__ ids, uint2* __restrict__ sorted,
 // ---------------------------------------------------------------------------------------
 
 constexpr int kReduceThreads = 256;
-constexpr int kInFlight = 8;                      // gradient rows a thread has under way
-
 template <int VEC> struct Piece;
 template <> struct Piece<4>
 {
@@ -416,6 +414,8 @@ embedding_chunk_kernel(const uint2* sorted, const unsigned char* present, const 
     __syncthreads();
     if(length == 0 || column >= E) return;
     const uint2* const item = items[which];
+    // gradient rows a thread has under way: 128 bytes of each input, fewer scalars (they cost a register each)
+    constexpr int kInFlight = VEC == 4 ? 8 : TWO ? 16 : 24;
     const long long end = start + length;
     const unsigned int before = start > 0 ? sorted[start - 1].x : 0xffffffffu, behind = end < tokens ? sorted[end].x : 0xffffffffu;
 
@@ -641,8 +641,10 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
 
     const bool vec = (E & 3) == 0 && host_aligned16(dY) && host_aligned16(dY2) && host_aligned16(dW);
     const int pieces = (int)(vec ? E / 4 : E);
-    int group = 32;
-    while(group < kReduceThreads && group < pieces) group *= 2;
+    // threads of a chunk: the widest group that leaves fewest of its threads without a column
+    int group = kReduceThreads;
+    for(int g = kReduceThreads / 2; g >= 32; g /= 2)
+        if((pieces + g - 1) / g * g < (pieces + group - 1) / group * group) group = g;
     const int chunk = chunk_of(tokens), groups = kReduceThreads / group;
     const int chunk_ctas = (l.chunks + groups - 1) / groups, zero_ctas = accumulate ? 0 : (int)((V + kZeroRows - 1) / kZeroRows);
     const dim3 grid((unsigned)(chunk_ctas + zero_ctas), (unsigned)((pieces + group - 1) / group));
