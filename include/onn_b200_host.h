@@ -100,6 +100,13 @@ int onn_trainer_step_host_i32(onn_trainer* trainer, const int32_t* decoder_ids, 
 /* NeuralNetwork::forward_propagate on one micro-batch of device-resident ids
  * (is_training = 0: the output layer holds probabilities). */
 int onn_trainer_forward(onn_trainer* trainer, const float* decoder_ids, const float* encoder_ids, int is_training);
+/* Scores tokens under the network: NeuralNetwork::forward_propagate on one micro-batch of device-resident ids, then
+ * onn_token_logprobs on the output layer's logits.  targets [micro_batch, decoder_sequence_length] (NULL: no logprobs, every
+ * position takes part); logprobs, entropy [rows] and top_ids, top_logprobs [rows, top] as in onn_token_logprobs, with
+ * rows = micro_batch * decoder_sequence_length; NULL for what is not wanted.  All are device pointers; the work runs on
+ * onn_trainer_stream() and is not waited for. */
+int onn_trainer_token_logprobs(onn_trainer* trainer, const float* decoder_ids, const float* encoder_ids, const float* targets,
+                               float temperature, float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, int64_t top);
 /* Greedy decoding on token ids: the loop of Transformer::calculate_outputs (opennn/standard_networks.cpp:1002-1035)
  * without the tokeniser and vocabulary maps around it.  encoder_ids (host, [micro_batch, input_sequence_length]) are
  * decoded independently row by row; decoded_ids (host, [micro_batch, decoder_sequence_length]) receives

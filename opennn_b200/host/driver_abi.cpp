@@ -994,6 +994,29 @@ extern "C" int onn_trainer_forward(onn_trainer* t, const float* decoder_ids, con
     });
 }
 
+extern "C" int onn_trainer_token_logprobs(onn_trainer* t, const float* decoder_ids, const float* encoder_ids, const float* targets,
+                                          float temperature, float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, int64_t top)
+{
+    if(!t || !decoder_ids || (!t->decoder_only && !encoder_ids)) return ONN_ERR_INVALID_ARGUMENT;
+    return guarded([&]
+    {
+        Device::instance().set_compute_stream(t->stream);
+        await_parameters(t);
+        BatchCuda micro;
+        micro.samples_number = t->micro_batch;
+        micro.decoder = TensorViewCuda(const_cast<float*>(decoder_ids), {t->micro_batch, t->decoder_sequence_length});
+        if(!t->decoder_only) micro.input = TensorViewCuda(const_cast<float*>(encoder_ids), {t->micro_batch, t->input_sequence_length});
+        auto* dense = dynamic_cast<Dense3dForwardPropagationCuda*>(t->forward->layers.back().get());
+        if(!dense || !dense->defer_softmax) throw std::runtime_error("onn_trainer_token_logprobs: the output layer does not leave logits.");
+        t->network->forward_propagate(micro.get_inputs_device(), *t->forward, true);     // as in training: the softmax is left to the reader
+        const TensorViewCuda logits = t->forward->get_last_trainable_layer_outputs_device();
+        const Index V = logits.shape.back();
+        const int status = onn_token_logprobs(logits.data, ONN_F32, V, targets, logprobs, entropy, nullptr, top_ids, top_logprobs, top,
+                                              logits.size() / V, V, temperature, t->stream);
+        if(status != ONN_OK) throw StatusError(status, string("onn_token_logprobs: ") + onn_status_string(status));
+    });
+}
+
 extern "C" int onn_trainer_greedy_decode(onn_trainer* t, const float* encoder_ids, float* decoded_ids, int start_id, int end_id)
 {
     if(!t || !encoder_ids || !decoded_ids || t->decoder_only) return ONN_ERR_INVALID_ARGUMENT;

@@ -24,7 +24,7 @@ HOST_EXPORTS = [
     "onn_trainer_get_gradients", "onn_trainer_set_learning_rate", "onn_trainer_set_iteration", "onn_trainer_set_dp",
     "onn_trainer_step_device", "onn_trainer_step_host", "onn_trainer_step_host_i32", "onn_trainer_forward", "onn_trainer_get_layer_output",
     "onn_trainer_synchronize", "onn_trainer_parameters_ready", "onn_trainer_exchange_segments", "onn_trainer_trace_phases", "onn_trainer_last_step_phases", "onn_trainer_stream", "onn_trainer_set_graph_capture", "onn_trainer_set_dp_options",
-    "onn_trainer_greedy_decode", "onn_trainer_greedy_decode_cached",
+    "onn_trainer_token_logprobs", "onn_trainer_greedy_decode", "onn_trainer_greedy_decode_cached",
     "onn_classifier_last_error", "onn_classifier_create", "onn_classifier_destroy", "onn_classifier_parameters_number",
     "onn_classifier_layers_number", "onn_classifier_layer_info", "onn_classifier_set_parameters", "onn_classifier_get_parameters",
     "onn_classifier_get_gradients", "onn_classifier_set_learning_rate", "onn_classifier_forward", "onn_classifier_step_device",
@@ -164,6 +164,26 @@ class Trainer:
 
     def forward(self, dec_ids, enc_ids, is_training=False):
         _check(host_lib().onn_trainer_forward(self._handle, capi.ptr(dec_ids), capi.ptr(enc_ids), int(is_training)), "forward")
+
+    def token_logprobs(self, dec_ids, enc_ids, targets=None, top=0, temperature=1.0):
+        """Scores targets under the network.  dec_ids, enc_ids, targets: torch CUDA float tensors of one micro-batch.  Returns
+        (logprobs, entropy [micro_batch, S_dec], top_ids, top_logprobs [micro_batch, S_dec, top]), None for what is not asked."""
+        import torch
+        shape = (self.micro_batch, self.S_dec)
+        if tuple(dec_ids.shape) != shape or (targets is not None and tuple(targets.shape) != shape):
+            raise capi.OnnError(f"token_logprobs: ids and targets of one micro-batch, {shape}, are needed")
+        if (enc_ids is None) != (self.kind == DECODER_ONLY) or (enc_ids is not None and tuple(enc_ids.shape) != (self.micro_batch, self.S_in)):
+            raise capi.OnnError("token_logprobs: encoder ids of one micro-batch are needed (none for a decoder-only network)")
+        empty = lambda *more, dtype=torch.float32: torch.empty(*shape, *more, dtype=dtype, device="cuda")  # noqa: E731
+        logprobs, entropy = None if targets is None else empty(), empty()
+        top_ids, top_logprobs = (empty(top, dtype=torch.int32), empty(top)) if top > 0 else (None, None)
+        here, there = torch.cuda.current_stream(), self.stream()
+        there.wait_stream(here)
+        _check(host_lib().onn_trainer_token_logprobs(self._handle, capi.ptr(dec_ids), capi.ptr(enc_ids), capi.ptr(targets),
+                                                     C.c_float(temperature), capi.ptr(logprobs), capi.ptr(entropy), capi.ptr(top_ids),
+                                                     capi.ptr(top_logprobs), C.c_int64(top)), "token_logprobs")
+        here.wait_stream(there)
+        return logprobs, entropy, top_ids, top_logprobs
 
     def greedy_decode(self, encoder_ids, start_id=2, end_id=3, cached=False):
         """encoder_ids: float32 numpy [micro_batch, S_in]; returns float32 numpy [micro_batch, S_dec].

@@ -728,6 +728,42 @@ def test_two_streams_at_once(capi):
                 assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("kind", ["transformer", "decoder"])
+def test_trainer_scores_tokens(capi, kind):
+    """The trainer's scores are the logarithms of the probabilities that its inference pass leaves in the output layer."""
+    from opennn_b200 import trainer
+    S_in, S_dec, V, B = 24, 16, 320, 4
+    decoder_only = kind == "decoder"
+    t = trainer.Trainer(trainer.DECODER_ONLY if decoder_only else trainer.TRANSFORMER, S_dec if decoder_only else S_in, S_dec, V, V, 128, 2, 256, 1, B)
+    try:
+        import numpy as np
+        rng = np.random.default_rng(3)
+        t.set_parameters((rng.standard_normal(t.parameters_number) * 0.08).astype(np.float32))
+        gen = generator(4)
+        dec, tgt = (torch.randint(1, V, (B, S_dec), generator=gen, device="cuda").float() for _ in range(2))
+        enc = None if decoder_only else torch.randint(1, V, (B, S_in), generator=gen, device="cuda").float()
+        tgt[1, 9:] = 0.0
+        given, entropy, ids, values = t.token_logprobs(dec, enc, tgt, top=5)
+        t.forward(dec, enc, is_training=False)
+        p = torch.from_numpy(t.layer_output(t.layers_number - 1)).cuda().view(B, S_dec, V).double()
+        active = tgt > 0
+        logp = p.log()
+        want = torch.where(active, logp.gather(2, tgt.long()[..., None])[..., 0], 0.0)
+        # the probabilities are rounded to fp32, after an exponential and a division of their own
+        torch.testing.assert_close(given.double(), want, rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(entropy.double(), torch.where(active, -(p * logp).sum(2), 0.0), rtol=1e-5, atol=1e-5)
+        assert torch.equal((ids == -1).all(2), ~active)
+        torch.testing.assert_close(values[active].double(), p.topk(5, dim=2).values.log()[active], rtol=1e-5, atol=1e-5)
+        _, all_entropy, _, _ = t.token_logprobs(dec, enc)
+        assert (all_entropy > 0).all()
+        with pytest.raises(capi.OnnError):
+            t.token_logprobs(dec, enc, tgt, top=500)
+        with pytest.raises(capi.OnnError):
+            t.token_logprobs(dec[:2], enc, tgt)
+    finally:
+        t.close()
+
+
 def test_wrapper_refusals(capi):
     x = torch.zeros(4, 10, device="cuda")
     t = torch.ones(4, device="cuda")
