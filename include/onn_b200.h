@@ -418,7 +418,7 @@ int onn_token_logprobs(const void* logits, int dtype, int64_t pitch, const float
  * may then be NULL too),
  *   dlogits_i = (d_logprob (1[i = token] - p_i) - d_entropy p_i (log p_i + entropy)) / temperature,
  * 0 on padding rows, rounded once to dtype.  dlogits (row r at dlogits + r * d_pitch elements) is overwritten; it may
- * be the logits themselves (same pitch), but must not overlap them in another way.  Elements between V and the pitch
+ * be the logits themselves (with the same pitch, another is refused), but must not overlap them in another way.  Elements between V and the pitch
  * are left as they are. */
 int onn_token_logprobs_bwd(const void* logits, int dtype, int64_t pitch, const float* tokens, const float* lse,
                            const float* entropy, const float* d_logprobs, const float* d_entropy,

@@ -316,6 +316,7 @@ distill3d_finish_kernel(const float* __restrict__ row_losses, const float* __res
     __shared__ float scratch[32];
     pdl_wait();
     float soft = 0.f, hard = 0.f, active = 0.f;
+#pragma unroll 8
     for(long long i = threadIdx.x; i < rows; i += blockDim.x)
     {
         soft += row_losses[i];
@@ -409,7 +410,7 @@ extern "C" int onn_distill3d_fwd_bwd(const void* logits, int dtype, int64_t pitc
     ONN_CHECK_ARG(logit_arguments_ok(logits, dtype, pitch, rows, V) && temperature_ok(temperature));
     ONN_CHECK_ARG(targets && teacher_ids && teacher_logits && stats && row_losses && top >= 1);
     ONN_CHECK_ARG(isfinite(soft_weight) && isfinite(hard_weight));
-    ONN_CHECK_ARG(!dlogits || logit_arguments_ok(dlogits, dtype, d_pitch, rows, V));
+    ONN_CHECK_ARG(!dlogits || (logit_arguments_ok(dlogits, dtype, d_pitch, rows, V) && gradient_place_ok(logits, pitch, dlogits, d_pitch)));
     if(top > ONN_TOP_MAX) return ONN_ERR_LIMIT;
     cudaStream_t s = (cudaStream_t)stream;
     int status;

@@ -220,6 +220,8 @@ inline bool logit_arguments_ok(const void* logits, int dtype, int64_t pitch, int
     return logits && dtype >= ONN_F32 && dtype <= ONN_F16 && V > 1 && V < (1LL << 31) - 4096 && pitch >= V &&
            rows > 0 && rows < (1LL << 27) && reinterpret_cast<uintptr_t>(logits) % logit_bytes(dtype) == 0;
 }
+// Gradients in the logits' place keep their rows' places.
+inline bool gradient_place_ok(const void* logits, int64_t pitch, const void* dlogits, int64_t d_pitch) { return logits != dlogits || pitch == d_pitch; }
 inline bool temperature_ok(float t) { return t > 0.f && t <= 1e6f && t >= 1e-6f; }
 
 }  // namespace onn

@@ -774,7 +774,7 @@ extern "C" int onn_token_logprobs_bwd(const void* logits, int dtype, int64_t pit
 {
     ONN_CHECK_ARG(logit_arguments_ok(logits, dtype, pitch, rows, V) && temperature_ok(temperature));
     ONN_CHECK_ARG(tokens && lse && d_logprobs && (entropy || !d_entropy));
-    ONN_CHECK_ARG(logit_arguments_ok(dlogits, dtype, d_pitch, rows, V));
+    ONN_CHECK_ARG(logit_arguments_ok(dlogits, dtype, d_pitch, rows, V) && gradient_place_ok(logits, pitch, dlogits, d_pitch));
     const float inverse = 1.0f / temperature;
     cudaStream_t s = (cudaStream_t)stream;
     switch(dtype)

@@ -36,7 +36,7 @@ def backward(L, logits=P, dtype=0, pitch=100, tokens=P, lse=P, entropy=P, d_logp
 
 @pytest.mark.parametrize("bad", [
     dict(logits=None), dict(tokens=None), dict(lse=None), dict(entropy=None), dict(d_logprobs=None), dict(out=None), dict(d_pitch=99),
-    dict(out=P + 2), dict(out=P + 1, dtype=2), dict(T=0.0), dict(rows=0), dict(dtype=7)])
+    dict(out=P + 2), dict(out=P + 1, dtype=2), dict(T=0.0), dict(rows=0), dict(dtype=7), dict(d_pitch=101)])
 def test_token_logprobs_bwd_refuses(L, bad):
     assert backward(L, **bad) == BAD
 
@@ -49,7 +49,7 @@ def distill(L, logits=P, dtype=0, pitch=100, targets=P, count=P, ids=P, values=P
 @pytest.mark.parametrize("bad", [
     dict(logits=None), dict(targets=None), dict(ids=None), dict(values=None), dict(top=0), dict(stats=None), dict(losses=None),
     dict(T=0.0), dict(T=float("nan")), dict(soft=float("nan")), dict(hard=float("inf")), dict(d_pitch=99), dict(out=P + 2),
-    dict(rows=0), dict(V=1)])
+    dict(rows=0), dict(V=1), dict(d_pitch=101)])
 def test_distill_refuses(L, bad):
     assert distill(L, **bad) == BAD
 
@@ -67,6 +67,16 @@ def embed(L, ids=P, dY=P, dY2=P, dW=P, B=2, S=3, E=8, V=10, workspace=P, flags=0
     dict(B=1 << 20, S=1 << 12), dict(flags=8)])
 def test_embedding_bwd_sorted_refuses(L, bad):
     assert embed(L, **bad) == BAD
+
+
+def test_embedding_bwd_sorted_workspace(L):
+    """Sizes do not need a GPU; a missing workspace is told from a bad argument."""
+    assert L.onn_embedding_bwd_sorted_workspace_floats(2, 3, 8, 10) == 0
+    floats = L.onn_embedding_bwd_sorted_workspace_floats(64, 256, 1024, 32000)
+    assert floats >= 2 * 64 * 256
+    assert L.onn_embedding_bwd_sorted_workspace_floats(0, 3, 8, 10) == 0
+    assert embed(L, B=64, S=256, E=1024, V=32000, workspace=None) == -4
+    assert embed(L, B=64, S=256, E=1024, V=32000, workspace=P + 4) == BAD
 
 
 def test_wrappers_refuse_host_tensors(built):

@@ -140,6 +140,20 @@ def test_token_logprobs(capi, rows, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V", [(5000, 301), (4000, 2047), (620, 9001), (640, 1500), (400, 60000)])
+def test_token_logprobs_many_rows(capi, rows, V, dtype):
+    """Rows enough to fill the GPU: one CTA or warp each, several rows one after the other in the same warp."""
+    x = make_logits(rows, V, dtype, pitch=V + 2, seed=V)
+    x[::7] = (x[::7] * 2).round() / 2                     # ties
+    x[3::11] = 1.5                                        # all equal
+    x[5::13, V // 3:] = -INF
+    tokens = make_tokens(rows, V)
+    tokens[rows // 3: rows // 3 + 50] = 0.0
+    for top in (0, 7, 64, 128):
+        check_logprobs(capi, x, tokens, top, 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("pitch,offset", [(0, 1), (1, 0), (5, 3), (64, 7), (3, 2)])
 @pytest.mark.parametrize("V", [6, 77, 4100, 20011])
 def test_token_logprobs_strides(capi, V, pitch, offset, dtype):
@@ -395,6 +409,23 @@ def test_distill(capi, rows, V, dtype):
         x = make_logits(rows, V, dtype, seed=V + top)
         ids, values = make_teacher(rows, V, top)
         check_distill(capi, x, make_tokens(rows, V), ids, values, T, a * scale, b * scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V", [(3000, 300), (700, 5003), (320, 20000), (320, 36001), (160, 90000)])
+def test_distill_many_rows(capi, rows, V, dtype):
+    """Rows enough to fill the GPU, at the lengths where the number of threads changes."""
+    x = make_logits(rows, V, dtype, seed=V)
+    x[3::11] = 1.5
+    x[5::13, V // 3:] = -INF
+    targets = make_tokens(rows, V)
+    targets[rows // 3: rows // 3 + 50] = 0.0
+    scale = 1024.0 if dtype == "f16" else 1.0
+    for top, T, a, b in ((12, 2.0, 0.5, 0.5), (128, 1.0, 0.5, 0.5)):
+        ids, values = make_teacher(rows, V, top)
+        # a teacher of tokens that the student keeps, or the loss is infinite
+        ids = torch.where(ids >= V // 3, ids % (V // 3), ids)
+        check_distill(capi, x, targets, ids, values, T, a * scale, b * scale)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
