@@ -139,16 +139,23 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
     float m = end_value > -INFINITY ? end_value : -INFINITY;
     float s = 0.f, s1 = 0.f;
     if(end_index >= 0) { s = exp2_approx((end_value - finite_anchor(m)) * c); s1 = exp2_approx((end_value - finite_anchor(m)) * kLog2E); }
-    const int batches = (cut.vectors + T * N - 1) / (T * N);
+    // whole batches need no look at the row's end, and their addresses differ by constants
+    const int batches = (cut.vectors + T * N - 1) / (T * N), whole = cut.vectors / (T * N);
+    const uint4* const mine_body = body + tid;
     for(int batch = 0; batch < batches; batch++)
     {
         uint4 v[N];
         float larger = m;
-#pragma unroll
-        for(int u = 0; u < N; u++)
+        const uint4* const at = mine_body + (size_t)batch * (T * N);
+        if(batch < whole)
         {
-            const int i = (batch * N + u) * T + tid;
-            v[u] = i < cut.vectors ? body[i] : L::lowest();
+#pragma unroll
+            for(int u = 0; u < N; u++) v[u] = at[u * T];
+        }
+        else
+        {
+#pragma unroll
+            for(int u = 0; u < N; u++) v[u] = (batch * N + u) * T + tid < cut.vectors ? at[u * T] : L::lowest();
         }
 #pragma unroll
         for(int u = 0; u < N; u++) larger = fmaxf(larger, L::max(v[u]));
@@ -224,36 +231,58 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
     {
         const float2 minus = make_float2(-M, -M), c2 = make_float2(c, c), c1 = make_float2(kLog2E, kLog2E);
         const float2 w2 = make_float2(weight, weight), w12 = make_float2(weight1, weight1);
+        auto gradients = [&](const uint4& v, float (&f)[VE])
+        {
+            L::unpack(v, f);
+#pragma unroll
+            for(int e = 0; e < VE; e += 2)
+            {
+                const float2 d = add2(make_float2(f[e], f[e + 1]), minus), d2 = mul2(d, c2);
+                float2 g = mul2(make_float2(exp2_approx(d2.x), exp2_approx(d2.y)), w2);
+                if(SETS == 2)
+                {
+                    const float2 d1 = mul2(d, c1);
+                    g = fma2(make_float2(exp2_approx(d1.x), exp2_approx(d1.y)), w12, g);
+                }
+                f[e] = g.x;
+                f[e + 1] = g.y;
+            }
+        };
+        uint4* const mine_out = reinterpret_cast<uint4*>(dx + cut.head) + tid;
         for(int batch = batches - 1; batch >= 0; batch--)
         {
             uint4 v[N];
-#pragma unroll
-            for(int u = 0; u < N; u++)
+            const uint4* const at = mine_body + (size_t)batch * (T * N);
+            if(batch < whole && together)
             {
-                const int i = (batch * N + u) * T + tid;
-                if(i < cut.vectors) v[u] = __ldcs(body + i);
-            }
+                uint4* const to = mine_out + (size_t)batch * (T * N);
 #pragma unroll
-            for(int u = 0; u < N; u++)
-            {
-                const int i = (batch * N + u) * T + tid;
-                if(i >= cut.vectors) continue;
-                float f[VE];
-                L::unpack(v[u], f);
+                for(int u = 0; u < N; u++) v[u] = __ldcs(at + u * T);
 #pragma unroll
-                for(int e = 0; e < VE; e += 2)
+                for(int u = 0; u < N; u++)
                 {
-                    const float2 d = add2(make_float2(f[e], f[e + 1]), minus), d2 = mul2(d, c2);
-                    float2 g = mul2(make_float2(exp2_approx(d2.x), exp2_approx(d2.y)), w2);
-                    if(SETS == 2)
-                    {
-                        const float2 d1 = mul2(d, c1);
-                        g = fma2(make_float2(exp2_approx(d1.x), exp2_approx(d1.y)), w12, g);
-                    }
-                    f[e] = g.x;
-                    f[e + 1] = g.y;
+                    float f[VE];
+                    gradients(v[u], f);
+                    __stcs(to + u * T, L::pack(f));
                 }
-                store(i, f);
+            }
+            else
+            {
+#pragma unroll
+                for(int u = 0; u < N; u++)
+                {
+                    const int i = (batch * N + u) * T + tid;
+                    if(i < cut.vectors) v[u] = __ldcs(at + u * T);
+                }
+#pragma unroll
+                for(int u = 0; u < N; u++)
+                {
+                    const int i = (batch * N + u) * T + tid;
+                    if(i >= cut.vectors) continue;
+                    float f[VE];
+                    gradients(v[u], f);
+                    store(i, f);
+                }
             }
         }
         if(end_index >= 0) L::put(dx + end_index, gradient(end_value));
