@@ -700,9 +700,10 @@ int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float*
 
 // Threads of a row.  What a row costs besides its logits (start, reductions, ranking) is latency, so short rows want many
 // small CTAs: one warp up to 512 vectors (16384 x 1000 fp32: 27 us against 47 with 128 threads, 91 with 256), as
-// long as its 64 samples give a bound for the list (top <= 32).  A list of a long row wants more samples: 256 threads from
-// 12288 vectors (2048 x 131072 fp32 with 64 alternatives: 187 us against 212), else 128 (8192 x 50021 bf16: 203 against
-// 232).  Few rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read.
+// long as its 64 samples give a bound for the list (top <= 32).  A long list of a long row wants more samples: 256 threads
+// from 12288 vectors and 33 alternatives (2048 x 131072 fp32 with 64: 187 us against 212; 8192 x 50021 fp32 with 1: 272
+// against 248), else 128 (8192 x 50021 bf16 with 64: 203 against 232).  Few rows: a row is shared by the CTAs of a cluster, as
+// long as each has two vectors per thread to read.
 template <int DTYPE>
 int launch_fwd(const void* logits, int64_t pitch, const float* tokens, float* logprobs, float* entropy, float* lse,
                int32_t* top_ids, float* top_logprobs, int64_t top, int64_t rows, int64_t V, float c, float inverse_temperature,
@@ -711,7 +712,7 @@ int launch_fwd(const void* logits, int64_t pitch, const float* tokens, float* lo
     const int64_t vectors = V / Logit<DTYPE>::VE;
     int ctas = 1;
     while(ctas < kMaxCluster && rows * ctas * 2 <= 4 * kSmCount && vectors >= (int64_t)ctas * 1024) ctas *= 2;
-    const int T = ctas > 1 || (top > 0 && vectors >= 12288) ? 256 : vectors <= 512 && top <= 32 ? 32 : 128;
+    const int T = ctas > 1 || (top > 32 && vectors >= 12288) ? 256 : vectors <= 512 && top <= 32 ? 32 : 128;
     const auto launch = top > 0 ? (T == 32 ? launch_fwd_as<DTYPE, true, 32> : T == 128 ? launch_fwd_as<DTYPE, true, 128> : launch_fwd_as<DTYPE, true, 256>)
                                 : (T == 32 ? launch_fwd_as<DTYPE, false, 32> : T == 128 ? launch_fwd_as<DTYPE, false, 128> : launch_fwd_as<DTYPE, false, 256>);
     return launch(logits, pitch, tokens, logprobs, entropy, lse, top_ids, top_logprobs, top, rows, V, c, inverse_temperature, ctas, stream);
