@@ -402,7 +402,7 @@ def check_distill(capi, x, targets, ids, values, T, a, b, out=None):
 @pytest.mark.parametrize("rows,V", [(1, 2), (5, 7), (4, 31), (3, 1000), (9, 1023), (5, 1025), (3, 4097), (2, 8193), (33, 8000), (5, 16384), (4, 16391),
                                     (3, 32000), (2, 50021), (3, 65537), (2, 131072), (1, 262147), (700, 515), (1, 530000)])
 def test_distill(capi, rows, V, dtype):
-    for top, T, a, b in ((1, 1.0, 1.0, 0.0), (8, 2.0, 0.5, 0.5), (64, 1.0, 0.3, 0.7), (128, 3.0, 1.0, 0.0), (5, 1.0, 0.0, 1.0)):
+    for top, T, a, b in ((1, 1.0, 1.0, 0.0), (8, 2.0, 0.5, 0.5), (64, 1.0, 0.3, 0.7), (128, 3.0, 1.0, 0.0), (5, 1.0, 0.0, 1.0), (16, 0.7, 0.5, 0.5)):
         if V > 100000 and top == 64:
             continue
         scale = 64.0 if dtype == "f16" else 1.0
@@ -421,7 +421,7 @@ def test_distill_many_rows(capi, rows, V, dtype):
     targets = make_tokens(rows, V)
     targets[rows // 3: rows // 3 + 50] = 0.0
     scale = 1024.0 if dtype == "f16" else 1.0
-    for top, T, a, b in ((12, 2.0, 0.5, 0.5), (128, 1.0, 0.5, 0.5)):
+    for top, T, a, b in ((12, 2.0, 0.5, 0.5), (128, 1.0, 0.5, 0.5), (30, 1.5, 0.7, 0.3)):
         ids, values = make_teacher(rows, V, top)
         # a teacher of tokens that the student keeps, or the loss is infinite
         ids = torch.where(ids >= V // 3, ids % (V // 3), ids)
@@ -475,7 +475,7 @@ def test_distill_lists_and_masks(capi, V, dtype):
     x[11, targets[11].long()] = -INF                               # the target masked
     x[12] = torch.finfo(x.dtype).min                               # all at the type's lowest value
     ids[13, 0], values[13, 0] = ids[13, 1], 40.0                   # the likeliest token stands twice
-    for T, a, b in ((1.0, 1.0, 0.0), (2.0, 0.5, 0.5), (1.0, 0.25, 0.75)):
+    for T, a, b in ((1.0, 1.0, 0.0), (2.0, 0.5, 0.5), (1.0, 0.25, 0.75), (1.5, 0.5, 0.5)):
         check_distill(capi, x, targets, ids, values, T, a, b)
     # NaN and +inf stay in their rows
     x[0, V // 2], x[1, 1], values[3, 1] = math.nan, INF, math.nan
