@@ -54,6 +54,19 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const typename L::type* x = logits + row * pitch;
     typename L::type* dx = dlogits ? dlogits + row * d_pitch : nullptr;
+    // the target and the teacher's list (all of it in the first warp) are asked for together
+    constexpr int kPlaces = ONN_TOP_MAX / 32;
+    int index = tid < top ? __ldg(teacher_ids + row * top + tid) : -1;
+    int id[kPlaces];
+    float u[kPlaces];
+#pragma unroll
+    for(int k = 0; k < kPlaces; k++)
+    {
+        const int at = k * 32 + lane;
+        const bool there = warp == 0 && at < top;
+        id[k] = there ? __ldg(teacher_ids + row * top + at) : -1;
+        u[k] = there ? __ldg(teacher_logits + row * top + at) : -INFINITY;
+    }
     bool active;
     const long long target = row_token(targets, row, V, &active);
 
@@ -84,49 +97,11 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
         return;
     }
     // thread k < top looks after place k of the list, thread `top` after the target
-    int index = -1;
-    if(tid < top) index = __ldg(teacher_ids + row * top + tid);
-    else if(tid == top) index = (int)target;
+    if(tid == top) index = (int)target;
     if(index < 0 || index >= V) index = -1;
     const float special_logit = index >= 0 ? L::get(x + index) : -INFINITY;
     const float end_value = end_index >= 0 ? L::get(x + end_index) : -INFINITY;
 
-    if(warp == 0)
-    {
-        // the teacher's softmax over the valid places
-        constexpr int kPlaces = ONN_TOP_MAX / 32;
-        float u[kPlaces], largest = -INFINITY;
-        int id[kPlaces];
-#pragma unroll
-        for(int k = 0; k < kPlaces; k++)
-        {
-            const int at = k * 32 + lane;
-            id[k] = at < top ? __ldg(teacher_ids + row * top + at) : -1;
-            if(id[k] < 0 || id[k] >= V) id[k] = -1;
-            u[k] = id[k] >= 0 ? __ldg(teacher_logits + row * top + at) : -INFINITY;
-            largest = fmaxf(largest, u[k]);
-        }
-        largest = finite_anchor(warp_max(largest));
-        float e[kPlaces], sum = 0.f;
-#pragma unroll
-        for(int k = 0; k < kPlaces; k++)
-        {
-            // NaN passes the maximum by: it comes in through the sum
-            e[k] = id[k] < 0 ? 0.f : exp2_approx((u[k] - largest) * (kLog2E * inverse_temperature));
-            sum += e[k];
-        }
-        sum = warp_sum(sum);
-        const float inverse = 1.f / sum, log_sum = logf(sum);
-#pragma unroll
-        for(int k = 0; k < kPlaces; k++)
-        {
-            const int at = k * 32 + lane;
-            shared.id[at] = id[k];
-            shared.q[at] = sum != 0.f && id[k] >= 0 ? e[k] * inverse : 0.f;
-            shared.log_q[at] = (u[k] - largest) * inverse_temperature - log_sum;
-        }
-        if(lane == 0) shared.taught = sum != 0.f;
-    }
     float counted = 0.f;
     if(!active_count)
     {
@@ -195,6 +170,38 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
         }
         s += s2.x + s2.y;
         s1 += s12.x + s12.y;
+    }
+    if(warp == 0)
+    {
+        // the teacher's softmax over the valid places
+        float largest = -INFINITY;
+#pragma unroll
+        for(int k = 0; k < kPlaces; k++)
+        {
+            if(id[k] < 0 || id[k] >= V) { id[k] = -1; u[k] = -INFINITY; }
+            largest = fmaxf(largest, u[k]);
+        }
+        largest = finite_anchor(warp_max(largest));
+        float e[kPlaces], sum = 0.f;
+#pragma unroll
+        for(int k = 0; k < kPlaces; k++)
+        {
+            // NaN passes the maximum by: it comes in through the sum
+            e[k] = id[k] < 0 ? 0.f : exp2_approx((u[k] - largest) * c);
+            sum += e[k];
+        }
+        sum = warp_sum(sum);
+        const float inverse = 1.f / sum, log_sum = logf(sum);
+#pragma unroll
+        for(int k = 0; k < kPlaces; k++)
+        {
+            const int at = k * 32 + lane;
+            shared.id[at] = id[k];
+            if(k * 32 >= top) continue;
+            shared.q[at] = sum != 0.f && id[k] >= 0 ? e[k] * inverse : 0.f;
+            shared.log_q[at] = (u[k] - largest) * inverse_temperature - log_sum;
+        }
+        if(lane == 0) shared.taught = sum != 0.f;
     }
     const float warp_m = warp_max(m);
     {
