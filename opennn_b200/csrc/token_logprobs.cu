@@ -140,7 +140,7 @@ struct alignas(16) Part { float m, s, w, top; };
 // Warps that share a row (clusters are of 256 threads), and candidates: a single warp has short rows and lists, and little shared
 // memory lets more of them run (16384 x 1000 fp32 with 20 alternatives: 39 us, with 1024 candidates 75).
 template <int T> constexpr int kMaxParts = T == 256 ? kMaxCluster * 8 : T / 32;
-template <int T> constexpr int kCandidates = T == 32 ? 256 : 1024;
+template <int T> constexpr int kCandidates = T == 32 ? 256 : T == 64 ? 512 : 1024;
 
 // Shared memory of a CTA of T threads.  `parts` and, in the first CTA of a cluster, `candidates` are written by the whole
 // cluster.
@@ -690,8 +690,8 @@ int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float*
     using L = Logit<DTYPE>;
     // eight vectors in flight per thread; in 16 bits with a list four: the row's units are finer, and 8 CTAs of 128 threads fit
     constexpr int N = DTYPE != ONN_F32 && TOP ? 4 : 8;
-    // single warps walk over the rows (27 us against 35 for 16384 rows of 1000 logits); larger CTAs have one row each, so that
-    // whoever is free takes the next (203 us against 213 for 8192 rows of 50021 with 64 alternatives)
+    // single warps walk over the rows (16384 x 1000 fp32: 27 us, one row each 35); larger CTAs have one row each, so that whoever is
+    // free takes the next (8192 x 50021 bf16 with 64 alternatives: 203 us, walking 213)
     int64_t clusters = rows;
     if(T == 32 && clusters > 24 * kSmCount) clusters = 24 * kSmCount;
     if(launch_clusters(token_logprobs_kernel<DTYPE, TOP, T, N>, (unsigned)(clusters * ctas), T, ctas, 0, false, stream,
@@ -702,11 +702,25 @@ int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float*
 }
 
 // Threads of a row.  What a row costs besides its logits (start, reductions, ranking) is latency, so short rows want many
-// small CTAs: one warp up to 512 vectors (16384 x 1000 fp32: 27 us against 47 with 128 threads, 91 with 256), as
-// long as its 64 samples give a bound for the list (top <= 32).  A long list of a long row wants more samples: 256 threads
-// from 12288 vectors and 33 alternatives (2048 x 131072 fp32 with 64: 187 us against 212; 8192 x 50021 fp32 with 1: 272
-// against 248), else 128 (8192 x 50021 bf16 with 64: 203 against 232).  Few rows: a row is shared by the CTAs of a cluster, as
-// long as each has two vectors per thread to read.
+// small CTAs; but the bound for a list comes from two samples of each thread, and a long list wants many.  In us:
+//                       alternatives     32      64     128     256 threads
+//   16384 x  4000 fp32            0       45      48      55      99
+//   16384 x  4000 fp32           20       68      87     113     199
+//   16384 x  4000 fp32           64              120     138     222
+//   16384 x  8000 bf16           32      110     103     132
+//    8192 x 16000 fp32            0       91      86      81      84
+//    8192 x 16000 fp32           20      116     113     105     150
+//    8192 x 32000 fp32           64              251     232     211
+//    8192 x 50021 bf16           64              244     199     222
+// Few rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read.
+int threads_of(int64_t vectors, int64_t top)
+{
+    if(top == 0) return vectors <= 2048 ? 32 : 128;
+    if(top <= 24 && vectors <= 1024) return 32;
+    if(top <= 64 && vectors <= 2048) return 64;
+    return top > 32 && vectors >= 7168 ? 256 : 128;
+}
+
 template <int DTYPE>
 int launch_fwd(const void* logits, int64_t pitch, const float* tokens, float* logprobs, float* entropy, float* lse,
                int32_t* top_ids, float* top_logprobs, int64_t top, int64_t rows, int64_t V, float c, float inverse_temperature,
@@ -715,8 +729,8 @@ int launch_fwd(const void* logits, int64_t pitch, const float* tokens, float* lo
     const int64_t vectors = V / Logit<DTYPE>::VE;
     int ctas = 1;
     while(ctas < kMaxCluster && rows * ctas * 2 <= 4 * kSmCount && vectors >= (int64_t)ctas * 1024) ctas *= 2;
-    const int T = ctas > 1 || (top > 32 && vectors >= 12288) ? 256 : vectors <= 512 && top <= 32 ? 32 : 128;
-    const auto launch = top > 0 ? (T == 32 ? launch_fwd_as<DTYPE, true, 32> : T == 128 ? launch_fwd_as<DTYPE, true, 128> : launch_fwd_as<DTYPE, true, 256>)
+    const int T = ctas > 1 ? 256 : threads_of(vectors, top);
+    const auto launch = top > 0 ? (T == 32 ? launch_fwd_as<DTYPE, true, 32> : T == 64 ? launch_fwd_as<DTYPE, true, 64> : T == 128 ? launch_fwd_as<DTYPE, true, 128> : launch_fwd_as<DTYPE, true, 256>)
                                 : (T == 32 ? launch_fwd_as<DTYPE, false, 32> : T == 128 ? launch_fwd_as<DTYPE, false, 128> : launch_fwd_as<DTYPE, false, 256>);
     return launch(logits, pitch, tokens, logprobs, entropy, lse, top_ids, top_logprobs, top, rows, V, c, inverse_temperature, ctas, stream);
 }
