@@ -170,20 +170,20 @@ def embedding_bwd(ids, dY, V, scale=True, dY2=None):
     return dW
 
 
-def _f32(t, shape, what):
-    """Address of a float tensor of a given shape (None = NULL)."""
+def _f32(t, shape, what, device):
+    """Address of a float tensor of so many elements on a device (None = NULL)."""
     if t is None:
         return None
-    if t.dtype is not torch.float32 or t.numel() != shape or not t.is_cuda or not t.is_contiguous():
-        raise OnnError(f"{what}: a contiguous float32 device tensor of {shape} elements is needed")
+    if t.dtype is not torch.float32 or t.numel() != shape or t.get_device() != device or not t.is_contiguous():
+        raise OnnError(f"{what}: a contiguous float32 tensor of {shape} elements on cuda:{device} is needed")
     return t.data_ptr()
 
 
-def _i32(t, shape, what):
+def _i32(t, shape, what, device):
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.numel() != shape or not t.is_cuda or not t.is_contiguous():
-        raise OnnError(f"{what}: a contiguous int32 device tensor of {shape} elements is needed")
+    if t.dtype is not torch.int32 or t.numel() != shape or t.get_device() != device or not t.is_contiguous():
+        raise OnnError(f"{what}: a contiguous int32 tensor of {shape} elements on cuda:{device} is needed")
     return t.data_ptr()
 
 
@@ -195,11 +195,11 @@ except ImportError:
 
 
 def _current_stream(t):
-    """The current stream, which has to be one of the device that holds t."""
+    """(current device, its current stream); the device has to be the one that holds t."""
     device = torch.cuda.current_device()
     if t.get_device() != device:
         raise OnnError(f"the tensors are on cuda:{t.get_device()}, the current device is cuda:{device}")
-    return _raw_stream(device)
+    return device, _raw_stream(device)
 
 
 def embedding_bwd_sorted(ids, dY, V, scale=True, dY2=None, dW=None, accumulate=False):
@@ -210,11 +210,11 @@ def embedding_bwd_sorted(ids, dY, V, scale=True, dY2=None, dW=None, accumulate=F
         dW = (torch.zeros if accumulate else torch.empty)(V, E, device="cuda")
     L = lib()
     n = B * S
-    stream = _current_stream(dY)
+    d, stream = _current_stream(dY)
     floats = L.onn_embedding_bwd_sorted_workspace_floats(B, S, E, V)
     workspace = _empty(floats) if floats else None
-    check(L.onn_embedding_bwd_sorted(_f32(ids, n, "ids"), _f32(dY, n * E, "dY"), _f32(dY2, n * E, "dY2"), _f32(dW, V * E, "dW"),
-                                     B, S, E, V, int(scale), _f32(workspace, floats, "workspace"), ACCUMULATE if accumulate else 0, stream),
+    check(L.onn_embedding_bwd_sorted(_f32(ids, n, "ids", d), _f32(dY, n * E, "dY", d), _f32(dY2, n * E, "dY2", d), _f32(dW, V * E, "dW", d),
+                                     B, S, E, V, int(scale), _f32(workspace, floats, "workspace", d), ACCUMULATE if accumulate else 0, stream),
           "onn_embedding_bwd_sorted")
     return dW
 
@@ -403,30 +403,31 @@ def token_logprobs(logits, tokens=None, top=0, temperature=1.0, out=None):
     [rows, top] in int32 and fp32; logprobs is None without tokens, the lists with top=0.  out: a tuple as returned,
     to be written again."""
     x, dtype, pitch, rows, V = _logit_rows(logits, "logits")
-    stream = _current_stream(logits)
+    d, stream = _current_stream(logits)
     if out is None:
         out = (None if tokens is None else _empty(rows), _empty(rows), _empty(rows),
                torch.empty(rows, top, dtype=torch.int32, device="cuda") if top > 0 else None,
                torch.empty(rows, top, device="cuda") if top > 0 else None)
     logprobs, entropy, lse, top_ids, top_logprobs = out
-    check(lib().onn_token_logprobs(x, dtype, pitch, _f32(tokens, rows, "tokens"), _f32(logprobs, rows, "logprobs"),
-                                   _f32(entropy, rows, "entropy"), _f32(lse, rows, "lse"), _i32(top_ids, rows * top, "top_ids"),
-                                   _f32(top_logprobs, rows * top, "top_logprobs"), top, rows, V, temperature, stream), "onn_token_logprobs")
+    check(lib().onn_token_logprobs(x, dtype, pitch, _f32(tokens, rows, "tokens", d), _f32(logprobs, rows, "logprobs", d),
+                                   _f32(entropy, rows, "entropy", d), _f32(lse, rows, "lse", d), _i32(top_ids, rows * top, "top_ids", d),
+                                   _f32(top_logprobs, rows * top, "top_logprobs", d), top, rows, V, temperature, stream), "onn_token_logprobs")
     return out
 
 
 def token_logprobs_bwd(logits, tokens, lse, entropy, d_logprobs, d_entropy=None, temperature=1.0, out=None):
     """The gradient of token_logprobs' logprobs and entropy with respect to the logits.  out may be the logits themselves."""
     x, dtype, pitch, rows, V = _logit_rows(logits, "logits")
+    d, stream = _current_stream(logits)
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     dx, d_dtype, d_pitch, d_rows, d_V = _logit_rows(out, "out")
-    if (d_dtype, d_rows, d_V) != (dtype, rows, V):
-        raise OnnError("out: the logits' shape and type are needed")
-    check(lib().onn_token_logprobs_bwd(x, dtype, pitch, _f32(tokens, rows, "tokens"), _f32(lse, rows, "lse"),
-                                       _f32(entropy, rows, "entropy"), _f32(d_logprobs, rows, "d_logprobs"),
-                                       _f32(d_entropy, rows, "d_entropy"), dx, d_pitch, rows, V, temperature,
-                                       _current_stream(logits)), "onn_token_logprobs_bwd")
+    if (d_dtype, d_rows, d_V) != (dtype, rows, V) or out.get_device() != d:
+        raise OnnError("out: the logits' shape, type and device are needed")
+    check(lib().onn_token_logprobs_bwd(x, dtype, pitch, _f32(tokens, rows, "tokens", d), _f32(lse, rows, "lse", d),
+                                       _f32(entropy, rows, "entropy", d), _f32(d_logprobs, rows, "d_logprobs", d),
+                                       _f32(d_entropy, rows, "d_entropy", d), dx, d_pitch, rows, V, temperature,
+                                       stream), "onn_token_logprobs_bwd")
     return out
 
 
@@ -436,18 +437,19 @@ def distill3d(logits, targets, teacher_ids, teacher_logits, temperature=1.0, sof
     loss.  Returns (stats {sum of soft, sum of hard, #active}, row losses [2, rows], gradient or None), all on the device.
     out: a tuple as returned, to be written again; its gradient may be the logits themselves."""
     x, dtype, pitch, rows, V = _logit_rows(logits, "logits")
+    d, stream = _current_stream(logits)
     top = teacher_ids.shape[-1]
     if out is None:
         out = (_empty(3), torch.empty(2, rows, device="cuda"),
                torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if want_gradient else None)
     stats, row_losses, gradient = out
     dx, d_dtype, d_pitch, d_rows, d_V = (None, dtype, V, rows, V) if gradient is None else _logit_rows(gradient, "gradient")
-    if (d_dtype, d_rows, d_V) != (dtype, rows, V):
-        raise OnnError("gradient: the logits' shape and type are needed")
-    check(lib().onn_distill3d_fwd_bwd(x, dtype, pitch, _f32(targets, rows, "targets"), _f32(active_count, 1, "active_count"),
-                                      _i32(teacher_ids, rows * top, "teacher_ids"), _f32(teacher_logits, rows * top, "teacher_logits"),
-                                      top, temperature, soft_weight, hard_weight, dx, d_pitch, _f32(stats, 3, "stats"),
-                                      _f32(row_losses, 2 * rows, "row_losses"), rows, V, _current_stream(logits)),
+    if (d_dtype, d_rows, d_V) != (dtype, rows, V) or (gradient is not None and gradient.get_device() != d):
+        raise OnnError("gradient: the logits' shape, type and device are needed")
+    check(lib().onn_distill3d_fwd_bwd(x, dtype, pitch, _f32(targets, rows, "targets", d), _f32(active_count, 1, "active_count", d),
+                                      _i32(teacher_ids, rows * top, "teacher_ids", d), _f32(teacher_logits, rows * top, "teacher_logits", d),
+                                      top, temperature, soft_weight, hard_weight, dx, d_pitch, _f32(stats, 3, "stats", d),
+                                      _f32(row_losses, 2 * rows, "row_losses", d), rows, V, stream),
           "onn_distill3d_fwd_bwd")
     return out
 

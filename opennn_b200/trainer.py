@@ -178,11 +178,16 @@ class Trainer:
         logprobs, entropy = None if targets is None else empty(), empty()
         top_ids, top_logprobs = (empty(top, dtype=torch.int32), empty(top)) if top > 0 else (None, None)
         here, there = torch.cuda.current_stream(), self.stream()
+        device, rows = here.device.index, self.micro_batch * self.S_dec
+        decoder, encoder = capi._f32(dec_ids, rows, "dec_ids", device), capi._f32(enc_ids, self.micro_batch * self.S_in, "enc_ids", device)
+        wanted = capi._f32(targets, rows, "targets", device)
         there.wait_stream(here)
-        _check(host_lib().onn_trainer_token_logprobs(self._handle, capi.ptr(dec_ids), capi.ptr(enc_ids), capi.ptr(targets),
-                                                     C.c_float(temperature), capi.ptr(logprobs), capi.ptr(entropy), capi.ptr(top_ids),
-                                                     capi.ptr(top_logprobs), C.c_int64(top)), "token_logprobs")
-        here.wait_stream(there)
+        try:
+            _check(host_lib().onn_trainer_token_logprobs(self._handle, C.c_void_p(decoder), C.c_void_p(encoder), C.c_void_p(wanted),
+                                                         C.c_float(temperature), capi.ptr(logprobs), capi.ptr(entropy), capi.ptr(top_ids),
+                                                         capi.ptr(top_logprobs), C.c_int64(top)), "token_logprobs")
+        finally:
+            here.wait_stream(there)
         return logprobs, entropy, top_ids, top_logprobs
 
     def greedy_decode(self, encoder_ids, start_id=2, end_id=3, cached=False):

@@ -90,3 +90,28 @@ def test_wrappers_refuse_host_tensors(built):
         capi.token_logprobs(x.double(), t)
     with pytest.raises(capi.OnnError):
         capi.distill3d(x, t, torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, 1))
+
+
+def test_tensors_of_another_device_are_refused(built):
+    import torch
+
+    from opennn_b200 import capi
+
+    class On:
+        """A tensor as the checks see it, on device `device`."""
+
+        def __init__(self, device, dtype):
+            self.device, self.dtype = device, dtype
+
+        numel = staticmethod(lambda: 4)
+        is_contiguous = staticmethod(lambda: True)
+        data_ptr = staticmethod(lambda: 64)
+
+        def get_device(self):
+            return self.device
+
+    assert capi._f32(On(1, torch.float32), 4, "tokens", 1) == 64 and capi._i32(On(0, torch.int32), 4, "ids", 0) == 64
+    for call in (lambda: capi._f32(On(1, torch.float32), 4, "tokens", 0), lambda: capi._f32(On(-1, torch.float32), 4, "tokens", 0),
+                 lambda: capi._i32(On(0, torch.int32), 4, "ids", 1), lambda: capi._f32(On(0, torch.float64), 4, "tokens", 0)):
+        with pytest.raises(capi.OnnError):
+            call()

@@ -805,3 +805,18 @@ def test_wrapper_refusals(capi):
                  lambda: capi.embedding_bwd_sorted(t, torch.zeros(2, 3, 8, device="cuda"), 10)):
         with pytest.raises(capi.OnnError):
             call()
+
+
+def test_trainer_refuses_ids_that_are_not_floats(capi):
+    from opennn_b200 import trainer
+    t = trainer.Trainer(trainer.DECODER_ONLY, 16, 16, 320, 320, 128, 2, 256, 1, 4)
+    try:
+        ids = torch.ones(4, 16, device="cuda")
+        for call in (lambda: t.token_logprobs(ids, None, ids.long()), lambda: t.token_logprobs(ids.int(), None, ids),
+                     lambda: t.token_logprobs(ids, None, torch.ones(16, 4, device="cuda").t()), lambda: t.token_logprobs(ids.cpu(), None, ids)):
+            with pytest.raises(capi.OnnError):
+                call()
+        t.token_logprobs(ids, None, ids)
+        torch.cuda.synchronize()
+    finally:
+        t.close()
