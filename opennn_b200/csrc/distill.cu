@@ -4,6 +4,13 @@
 //   q = softmax over the valid places of u / T     p = softmax(x / T)     p1 = softmax(x)
 //   soft = T^2 sum_k q_k (log q_k - log p_{id_k})   hard = -log(p1_target + FLT_EPSILON)
 //   dx_i = [ soft_weight T (p_i - sum over k with id_k = i of q_k) + hard_weight (p1_i - 1[i = target]) ] / #active
+//
+// Bound by HBM at one read and one write of each logit: DRAM traffic is that (0.30 GB read for 0.30 GB of logits), the second
+// sweep comes from L1 (45 % of all loads) and L2.  Measured on a B200 (copy bandwidth 6.57 TB/s): 16384 x 32000 fp32 with both
+// parts at temperature 2, 37 % of the rows padding, 585 us = 5.8 TB/s; 4096 x 131072 bf16 with the soft part 419 us = 5.1 TB/s,
+// where the exponentials (two per logit, 16 per clock and SM) take 238 us by themselves.  Holding the row on chip instead was
+// slower: in the registers of a cluster of CTAs 789 and 776 us, in a persistent cluster with the next row's copies under way
+// 1163 and 1220 us (a cluster barrier and some 500 instructions per thread and row had nothing to hide behind).
 #include <float.h>
 
 #include <type_traits>
