@@ -16,8 +16,9 @@
 // Few positions take one launch instead: every CTA owns some rows of the table and looks for their ids itself.
 //
 // Measured on a B200 (copy bandwidth 6.57 TB/s): 128 x 1024 positions of 1024 features and two inputs, frequencies 1/v over
-// 50021 tokens, 250 us: sort 25, chunks 198 (1.28 GB: 6.5 TB/s), joins 17.  64 x 256 positions over 32000 tokens, 42 us: 6, 30
-// (173 MB: 5.8 TB/s), 6.  32 x 32 positions of 64 features: 3.6 us.
+// 50021 tokens, 247 us: sort 25, chunks 198 (1.28 GB: 6.5 TB/s), joins 14.  64 x 256 positions over 32000 tokens, 42 us: 6, 30
+// (173 MB: 5.8 TB/s), 6.  32 x 32 positions of 64 features and 1000
+// tokens: 3.3 us, 7 at frequencies 1/v.
 #include "common.cuh"
 #include "launch_counter.h"
 
@@ -36,7 +37,7 @@ constexpr int kOwnerWarps = kOwnerThreads / 32;
 constexpr int kTile = 1024;                       // ids looked at together
 constexpr int kOwnerColumns = 64;
 constexpr int kOwnerGroups = kOwnerThreads / kOwnerColumns;
-constexpr int kOwnerInFlight = 16;                // gradient elements a thread has under way
+constexpr int kOwnerInFlight = 16;                // gradient elements a thread has under way, of one input at a time
 constexpr int kMaxOwned = 32;                     // rows of a CTA, summed in shared memory
 
 // CTA (x, y) owns `owned` consecutive rows of the table, 64 columns of them.  It walks over all ids in order and keeps those that
@@ -100,26 +101,42 @@ embedding_owner_kernel(const float* __restrict__ ids, const float* __restrict__ 
         __syncthreads();
         if(column < E)
         {
+            // equal ids one after the other are added in a register
+            int current = -1;
+            float sum = 0.f;
             for(int i = group; i < total; i += kOwnerGroups * kOwnerInFlight)
             {
                 float g[kOwnerInFlight];
+                const float* from[kOwnerInFlight];
 #pragma unroll
                 for(int k = 0; k < kOwnerInFlight; k++)
                 {
                     const int j = i + k * kOwnerGroups;
-                    g[k] = 0.f;
-                    if(j >= total) continue;
-                    const long long at = (long long)(first + list_token[j]) * E + column;
-                    g[k] = __ldg(dY + at);
-                    if(dY2) g[k] += __ldg(dY2 + at);
+                    from[k] = dY + (long long)(first + (j < total ? list_token[j] : 0)) * E + column;
+                    g[k] = j < total ? __ldg(from[k]) : 0.f;
+                }
+                if(dY2)
+                {
+#pragma unroll
+                    for(int k = 0; k < kOwnerInFlight; k++)
+                        if(i + k * kOwnerGroups < total) g[k] += __ldg(dY2 + (from[k] - dY));
                 }
 #pragma unroll
                 for(int k = 0; k < kOwnerInFlight; k++)
                 {
                     const int j = i + k * kOwnerGroups;
-                    if(j < total) sums[group][list_row[j]][in_group] += g[k];
+                    if(j >= total) break;
+                    const int row = list_row[j];
+                    if(row != current)
+                    {
+                        if(current >= 0) sums[group][current][in_group] += sum;
+                        current = row;
+                        sum = 0.f;
+                    }
+                    sum += g[k];
                 }
             }
+            if(current >= 0) sums[group][current][in_group] += sum;
         }
     }
     __syncthreads();
@@ -473,7 +490,8 @@ embedding_chunk_kernel(const uint2* sorted, const unsigned char* present, const 
 
 // A run that starts in one chunk and goes on in the next ones: the second partial of its first chunk, then the first of each
 // following one.  A CTA adds 32 * VEC columns of a long run: its eight warps take every eighth part, and their sums are added
-// in order.  A warp adds a short one, four blocks of 32 * VEC columns at a time.
+// in order.  A warp adds a short one, four blocks of 32 * VEC columns at a time.  Short ones
+// are dealt out from the first CTA on, long ones from the last, so that few CTAs have both.
 template <int VEC>
 __global__ void __launch_bounds__(kReduceThreads)
 embedding_join_kernel(const uint2* sorted, const float* partial, const int2* owners, const int* control, float* __restrict__ dW,
@@ -491,7 +509,7 @@ embedding_join_kernel(const uint2* sorted, const float* partial, const int2* own
     auto part = [&](int index, int j, int column) { return P::load(partial + ((long long)(index + j) * 2 + (j == 0 ? 1 : 0)) * E + column); };
 
     const long long long_items = (long long)control[1] * blocks;
-    for(long long i = blockIdx.x; i < long_items; i += gridDim.x)
+    for(long long i = gridDim.x - 1 - blockIdx.x; i < long_items; i += gridDim.x)
     {
         const int2 owner = owners[chunks - 1 - i / blocks];
         const int index = owner.x, column = ((int)(i % blocks) * 32 + lane) * VEC;
@@ -530,7 +548,7 @@ embedding_join_kernel(const uint2* sorted, const float* partial, const int2* own
     }
 
     const int short_items = control[0];
-    for(int i = blockIdx.x + warp * gridDim.x; i < short_items; i += gridDim.x * kWarps)
+    for(int i = blockIdx.x * kWarps + warp; i < short_items; i += gridDim.x * kWarps)
     {
         const int2 owner = owners[i];
         const int index = owner.x;
