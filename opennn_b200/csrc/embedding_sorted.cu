@@ -16,9 +16,8 @@
 // Few positions take one launch instead: every CTA owns some rows of the table and looks for their ids itself.
 //
 // Measured on a B200 (copy bandwidth 6.57 TB/s): 128 x 1024 positions of 1024 features and two inputs, frequencies 1/v over
-// 50021 tokens, 247 us: sort 25, chunks 198 (1.28 GB: 6.5 TB/s), joins 14.  64 x 256 positions over 32000 tokens, 42 us: 6, 30
-// (173 MB: 5.8 TB/s), 6.  32 x 32 positions of 64 features and 1000
-// tokens: 3.3 us, 7 at frequencies 1/v.
+// 50021 tokens, 243 us: sort 25, chunks 198 (1.28 GB: 6.5 TB/s), joins the rest.  64 x 256 positions over 32000 tokens, 43 us: 6, 30
+// (173 MB: 5.8 TB/s), 6.  32 x 32 positions of 64 features and 1000 tokens: 3.3 us, 7 at frequencies 1/v.
 #include "common.cuh"
 #include "launch_counter.h"
 
@@ -43,7 +42,7 @@ constexpr int kMaxOwned = 32;                     // rows of a CTA, summed in sh
 // CTA (x, y) owns `owned` consecutive rows of the table, 64 columns of them.  It walks over all ids in order and keeps those that
 // are its own (in order: prefix sums); four groups of 64 threads, one per column, add every fourth of their gradient
 // rows each, and the groups' sums are added in order.
-__global__ void __launch_bounds__(kOwnerThreads)
+__global__ void __launch_bounds__(kOwnerThreads, 3)
 embedding_owner_kernel(const float* __restrict__ ids, const float* __restrict__ dY, const float* __restrict__ dY2,
                        float* __restrict__ dW, int tokens, int E, int V, float scale, int owned, int accumulate)
 {
@@ -107,19 +106,19 @@ embedding_owner_kernel(const float* __restrict__ ids, const float* __restrict__ 
             for(int i = group; i < total; i += kOwnerGroups * kOwnerInFlight)
             {
                 float g[kOwnerInFlight];
-                const float* from[kOwnerInFlight];
+                int at[kOwnerInFlight];
 #pragma unroll
                 for(int k = 0; k < kOwnerInFlight; k++)
                 {
                     const int j = i + k * kOwnerGroups;
-                    from[k] = dY + (long long)(first + (j < total ? list_token[j] : 0)) * E + column;
-                    g[k] = j < total ? __ldg(from[k]) : 0.f;
+                    at[k] = first + (j < total ? list_token[j] : 0);
+                    g[k] = j < total ? __ldg(dY + (long long)at[k] * E + column) : 0.f;
                 }
                 if(dY2)
                 {
 #pragma unroll
                     for(int k = 0; k < kOwnerInFlight; k++)
-                        if(i + k * kOwnerGroups < total) g[k] += __ldg(dY2 + (from[k] - dY));
+                        if(i + k * kOwnerGroups < total) g[k] += __ldg(dY2 + (long long)at[k] * E + column);
                 }
 #pragma unroll
                 for(int k = 0; k < kOwnerInFlight; k++)
@@ -141,15 +140,33 @@ embedding_owner_kernel(const float* __restrict__ ids, const float* __restrict__ 
     }
     __syncthreads();
     if(column >= E) return;
-    for(int v = v0 + group; v < v1; v += kOwnerGroups)
+    auto sum_of = [&](int r)
     {
-        float* to = dW + (long long)v * E + column;
-        float sum = sums[0][v - v0][in_group];
+        float sum = sums[0][r][in_group];
 #pragma unroll
-        for(int q = 1; q < kOwnerGroups; q++) sum += sums[q][v - v0][in_group];
-        sum *= scale;
-        if(!accumulate) *to = sum;
-        else if(present[v - v0]) *to += sum;
+        for(int q = 1; q < kOwnerGroups; q++) sum += sums[q][r][in_group];
+        return sum * scale;
+    };
+    float* const to = dW + (long long)v0 * E + column;
+    if(!accumulate)
+    {
+        for(int r = group; r < v1 - v0; r += kOwnerGroups) to[(long long)r * E] = sum_of(r);
+        return;
+    }
+    // the rows' earlier values are asked for together
+    constexpr int kRows = kMaxOwned / kOwnerGroups;
+    float earlier[kRows];
+#pragma unroll
+    for(int k = 0; k < kRows; k++)
+    {
+        const int r = group + k * kOwnerGroups;
+        earlier[k] = r < v1 - v0 && present[r] ? to[(long long)r * E] : 0.f;
+    }
+#pragma unroll
+    for(int k = 0; k < kRows; k++)
+    {
+        const int r = group + k * kOwnerGroups;
+        if(r < v1 - v0 && present[r]) to[(long long)r * E] = earlier[k] + sum_of(r);
     }
 }
 
@@ -384,59 +401,57 @@ __device__ __forceinline__ void put_row(float* to, typename Piece<VEC>::type sum
 constexpr int kLongRun = 4;                       // a run that crosses more chunk edges is long
 
 constexpr int kMaxChunk = 64;
+constexpr int kTree = 8;                          // gradient rows of one token that are added in pairs
 constexpr int kZeroRows = 32;                     // table rows of a CTA that writes zeros
 
-template <int VEC>
-__device__ void zero_absent_rows(const unsigned char* present, float* __restrict__ dW, int E, int V, long long v0)
+// A warp writes a row, or a part of it a short one, in 16-byte pieces between the row's ends.
+__device__ __forceinline__ void zero_absent_rows(const unsigned char* present, float* __restrict__ dW, int E, int V, long long v0)
 {
-    using P = Piece<VEC>;
-    const int pieces = E / VEC, tid = threadIdx.x;
-    const int rows = (int)(V - v0 < kZeroRows ? V - v0 : kZeroRows);
-    if(pieces >= 32)
+    int width = 32;
+    while(width > 4 && width * 2 >= E) width >>= 1;
+    const int lane = threadIdx.x & (width - 1);
+    for(int r = threadIdx.x / width; r < kZeroRows && v0 + r < V; r += kReduceThreads / width)
     {
-        for(int r = tid >> 5; r < rows; r += kReduceThreads / 32)
-        {
-            if(present[v0 + r]) continue;
-            for(int e = tid & 31; e < pieces; e += 32) P::store(dW + (v0 + r) * E + e * VEC, P::zero());
-        }
-    }
-    else
-    {
-        for(int i = tid; i < rows * pieces; i += kReduceThreads)
-            if(!present[v0 + i / pieces]) P::store(dW + v0 * E + (long long)i * VEC, P::zero());
+        if(present[v0 + r]) continue;
+        float* const row = dW + (v0 + r) * E;
+        const int head = min((int)((-reinterpret_cast<intptr_t>(row)) & 15) / 4, E), pieces = (E - head) / 4, after = head + pieces * 4;
+        if(lane < head) row[lane] = 0.f;
+        for(int i = lane; i < pieces; i += width) st4(row + head + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+        if(lane < E - after) row[after + lane] = 0.f;
     }
 }
 
 // A group of `group` threads adds one chunk, group * VEC columns of it.  control = {short runs to join, long ones, sorted positions}.
-// CTAs behind the first `chunk_ctas` write zeros.
+// CTAs behind the first chunk_ctas * across write zeros; the `across` CTAs that have a chunk's columns lie side by side.
 template <int VEC, bool TWO>
 __global__ void __launch_bounds__(kReduceThreads, TWO ? 2 : 3)
 embedding_chunk_kernel(const uint2* sorted, const unsigned char* present, const float* __restrict__ dY, const float* __restrict__ dY2,
                        float* __restrict__ dW, float* __restrict__ partial, int2* __restrict__ owners, int* control,
-                       int E, int V, int chunk, int chunks, int chunk_ctas, int group, float scale, int accumulate)
+                       int E, int V, int chunk, int chunks, int chunk_ctas, int across, int group, float scale, int accumulate)
 {
     using P = Piece<VEC>;
     using T = typename P::type;
     __shared__ uint2 items[kReduceThreads / 32][kMaxChunk];
     pdl_launch_dependents();
     pdl_wait();
-    if((int)blockIdx.x >= chunk_ctas)
+    const unsigned int along = blockIdx.x / across;
+    if(along >= (unsigned int)chunk_ctas)
     {
-        if(blockIdx.y == 0) zero_absent_rows<VEC>(present, dW, E, V, (long long)(blockIdx.x - chunk_ctas) * kZeroRows);
+        zero_absent_rows(present, dW, E, V, (long long)(blockIdx.x - chunk_ctas * across) * kZeroRows);
         return;
     }
     const int which = threadIdx.x / group;
-    const int index = blockIdx.x * (kReduceThreads / group) + which;
+    const int index = along * (kReduceThreads / group) + which;
     const int tokens = control[2];
-    const int column = (blockIdx.y * group + threadIdx.x % group) * VEC;
+    const int column = ((blockIdx.x - along * across) * group + threadIdx.x % group) * VEC;
     const long long start = (long long)index * chunk;
     const int length = (int)(start < tokens ? (tokens - start < chunk ? tokens - start : chunk) : 0);
     for(int i = threadIdx.x % group; i < length; i += group) items[which][i] = sorted[start + i];
     __syncthreads();
     if(length == 0 || column >= E) return;
     const uint2* const item = items[which];
-    // gradient rows a thread has under way: 128 bytes of each input, fewer scalars (they cost a register each)
-    constexpr int kInFlight = VEC == 4 ? 8 : TWO ? 16 : 24;
+    // gradient rows a thread has under way: 128 bytes of each input, 16 scalars (they cost a register each)
+    constexpr int kInFlight = VEC == 4 ? 8 : 16;
     const long long end = start + length;
     const unsigned int before = start > 0 ? sorted[start - 1].x : 0xffffffffu, behind = end < tokens ? sorted[end].x : 0xffffffffu;
 
@@ -471,18 +486,39 @@ embedding_chunk_kernel(const uint2* sorted, const unsigned char* present, const 
             if(TWO) other[u] = P::load(dY2 + at);
         }
 #pragma unroll
-        for(int u = 0; u < kInFlight; u++)
+        for(int u0 = 0; u0 < kInFlight; u0 += kTree)
         {
-            if(i + u >= length) break;
-            const unsigned int v = item[i + u].x;
-            if(v != current)
+            if(TWO)
             {
-                finish(true);
-                current = v;
-                starts_here = true;
-                sum = P::zero();
+#pragma unroll
+                for(int u = u0; u < u0 + kTree; u++) row[u] = P::add(row[u], other[u]);
             }
-            sum = P::add(sum, TWO ? P::add(row[u], other[u]) : row[u]);
+            if(i + u0 + kTree <= length && item[i + u0].x == current && item[i + u0 + kTree - 1].x == current)
+            {
+                // eight of a run: in pairs, for a smaller rounding error where runs are long
+#pragma unroll
+                for(int d = 1; d < kTree; d *= 2)
+                {
+#pragma unroll
+                    for(int u = u0; u < u0 + kTree; u += 2 * d) row[u] = P::add(row[u], row[u + d]);
+                }
+                sum = P::add(sum, row[u0]);
+                continue;
+            }
+#pragma unroll
+            for(int u = u0; u < u0 + kTree; u++)
+            {
+                if(i + u >= length) break;
+                const unsigned int v = item[i + u].x;
+                if(v != current)
+                {
+                    finish(true);
+                    current = v;
+                    starts_here = true;
+                    sum = P::zero();
+                }
+                sum = P::add(sum, row[u]);
+            }
         }
     }
     finish(behind != current);
@@ -508,11 +544,12 @@ embedding_join_kernel(const uint2* sorted, const float* partial, const int2* own
     // part 0 of a run is its first chunk's, part j that of the j-th behind it
     auto part = [&](int index, int j, int column) { return P::load(partial + ((long long)(index + j) * 2 + (j == 0 ? 1 : 0)) * E + column); };
 
-    const long long long_items = (long long)control[1] * blocks;
-    for(long long i = gridDim.x - 1 - blockIdx.x; i < long_items; i += gridDim.x)
+    const int long_runs = control[1];
+    int run = (int)(gridDim.x - 1 - blockIdx.x) / blocks, block = (int)(gridDim.x - 1 - blockIdx.x) % blocks;
+    for(; run < long_runs; run += (int)gridDim.x / blocks)
     {
-        const int2 owner = owners[chunks - 1 - i / blocks];
-        const int index = owner.x, column = ((int)(i % blocks) * 32 + lane) * VEC;
+        const int2 owner = owners[chunks - 1 - run];
+        const int index = owner.x, column = (block * 32 + lane) * VEC;
         const unsigned int v = (unsigned int)owner.y;
         int parts = 1;
         while(true)
@@ -544,6 +581,8 @@ embedding_join_kernel(const uint2* sorted, const float* partial, const int2* own
             for(int q = 1; q < kWarps; q++) sum = P::add(sum, warp_sums[q][lane]);
             put_row<VEC>(dW + (long long)v * E + column, sum, scale, accumulate);
         }
+        block += (int)gridDim.x % blocks;
+        if(block >= blocks) { block -= blocks; run++; }
         __syncthreads();
     }
 
@@ -669,12 +708,14 @@ extern "C" int onn_embedding_bwd_sorted(const float* ids, const float* dY, const
         if((pieces + g - 1) / g * g < (pieces + group - 1) / group * group) group = g;
     const int chunk = chunk_of(tokens), groups = kReduceThreads / group;
     const int chunk_ctas = (l.chunks + groups - 1) / groups, zero_ctas = accumulate ? 0 : (int)((V + kZeroRows - 1) / kZeroRows);
-    const dim3 grid((unsigned)(chunk_ctas + zero_ctas), (unsigned)((pieces + group - 1) / group));
+    const int across = (pieces + group - 1) / group;
+    const int64_t grid = (int64_t)chunk_ctas * across + zero_ctas;
+    if(grid >= 1LL << 31) return ONN_ERR_LIMIT;
     auto add = [&](auto kernel)
     {
-        return launch_overlapped(kernel, grid, dim3(kReduceThreads), 0, s, (const uint2*)sorted,
+        return launch_overlapped(kernel, dim3((unsigned)grid), dim3(kReduceThreads), 0, s, (const uint2*)sorted,
                                  (const unsigned char*)present, dY, dY2, dW, partial, owners, control, (int)E, (int)V, chunk, l.chunks,
-                                 chunk_ctas, group, scale_value, accumulate);
+                                 chunk_ctas, across, group, scale_value, accumulate);
     };
     cudaError_t error = vec ? (dY2 ? add(embedding_chunk_kernel<4, true>) : add(embedding_chunk_kernel<4, false>))
                             : (dY2 ? add(embedding_chunk_kernel<1, true>) : add(embedding_chunk_kernel<1, false>));

@@ -820,3 +820,49 @@ def test_trainer_refuses_ids_that_are_not_floats(capi):
         torch.cuda.synchronize()
     finally:
         t.close()
+
+
+@pytest.mark.parametrize("E", [3, 5, 14, 17, 62, 66, 130, 793])
+@pytest.mark.parametrize("offset", [0, 1, 2])
+def test_embedding_bwd_sorted_writes_every_absent_row(capi, E, offset):
+    """Rows of any length and alignment that do not occur: all of their elements, and nothing around the table."""
+    V, n = 4000, 2100
+    gen = generator(E)
+    room = torch.full((V * E + 8,), 7.0, device="cuda")
+    dW = room[offset:offset + V * E].view(V, E)
+    ids = torch.randint(1, 60, (1, n), generator=gen, device="cuda").float() * 50
+    dY = torch.randn(1, n, E, generator=gen, device="cuda")
+    capi.embedding_bwd_sorted(ids, dY, V, dW=dW)
+    want = torch.zeros(V, E, dtype=torch.float64, device="cuda").index_add_(0, ids.view(-1).long(), dY[0].double()) * math.sqrt(E)
+    absent = torch.ones(V, dtype=torch.bool, device="cuda")
+    absent[ids.view(-1).long()] = False
+    assert (dW[absent] == 0).all()
+    size = torch.zeros(V, E, dtype=torch.float64, device="cuda").index_add_(0, ids.view(-1).long(), dY[0].double().abs()) * math.sqrt(E)
+    count = torch.bincount(ids.view(-1).long(), minlength=V)[:, None]
+    # at most count + 2 roundings, each of at most half a step of a partial sum that the sum of the sizes bounds
+    assert ((dW.double() - want).abs() <= (count + 2) * 2.0 ** -24 * size).all()
+    assert (room[:offset] == 7).all() and (room[offset + V * E:] == 7).all()
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("two", [False, True])
+def test_embedding_bwd_sorted_small_tables_of_repeated_ids(capi, two, accumulate):
+    """The kernel for few positions with runs of equal ids, both inputs and earlier values."""
+    V, n, E = 90, 2048, 70
+    gen = generator(11)
+    ids = torch.where(torch.rand(1, n, generator=gen, device="cuda") < 0.5, torch.tensor(5.0, device="cuda"),
+                      torch.randint(0, V, (1, n), generator=gen, device="cuda").float())
+    dY, dY2 = (torch.randn(1, n, E, generator=gen, device="cuda") for _ in range(2))
+    before = torch.randn(V, E, generator=gen, device="cuda")
+    dW = before.clone()
+    capi.embedding_bwd_sorted(ids, dY, V, dY2=dY2 if two else None, dW=dW, accumulate=accumulate)
+    g = dY[0].double() + (dY2[0].double() if two else 0.0)
+    want = torch.zeros(V, E, dtype=torch.float64, device="cuda").index_add_(0, ids.view(-1).long(), g)
+    size = torch.zeros(V, E, dtype=torch.float64, device="cuda").index_add_(0, ids.view(-1).long(), g.abs()) * math.sqrt(E)
+    want, count = want * math.sqrt(E), torch.bincount(ids.view(-1).long(), minlength=V)[:, None]
+    want[0] = 0
+    size[0] = 0
+    if accumulate:
+        want, size = want + before.double(), size + before.double().abs()
+    # at most count + 4 roundings, each of at most half a step of a partial sum that the sum of the sizes bounds
+    assert ((dW.double() - want).abs() <= (count + 4) * 2.0 ** -24 * size + 1e-30).all()
