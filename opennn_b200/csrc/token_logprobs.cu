@@ -118,15 +118,15 @@ __device__ __forceinline__ float key_logit(unsigned long long key)
     return __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// A value that at least k of the lanes' pairs of logits (first >= second) reach: the largest is taken away k times.  Equal
-// ones of several lanes go together, which only lowers the result.
+// The k-th largest of the lanes' pairs of logits (first >= second): the largest ones are taken away until k are gone.
 __device__ __forceinline__ float warp_reached_by(float first, float second, int k)
 {
     float t;
     while(true)
     {
         asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(t) : "f"(first));
-        if(--k == 0) return t;
+        k -= __popc(__ballot_sync(0xffffffffu, first == t));
+        if(k <= 0) return t;
         if(first == t) { first = second; second = -INFINITY; }
     }
 }
@@ -340,7 +340,21 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     part.w = warp_sum(r.w);
     const int parts = ctas * kWarps;
     const int wanted = TOP ? (top + parts - 1) / parts : 1;
-    part.top = TOP ? warp_reached_by(best, second, wanted) : 0.f;
+    part.top = 0.f;
+    if constexpr(TOP)
+    {
+        // places that this warp has to vouch for: an equal share, or, in a row of so few vectors that the warps' numbers of them
+        // differ, one in proportion (2400 x 1600 bf16, 128 alternatives: 31 us, with equal shares 122, where
+        // a third of such a row became candidates)
+        int vouched = wanted;
+        if(each <= 2 && cut.vectors > 0)
+        {
+            auto of_warp = [&](int n) { return n < 0 ? 0 : n > 32 ? 32 : n; };
+            const int mine = of_warp(end - begin - warp * 32) + of_warp(end - begin - T - warp * 32);
+            vouched = (top * mine + cut.vectors - 1) / cut.vectors;
+        }
+        part.top = vouched > 0 ? warp_reached_by(best, second, vouched) : INFINITY;
+    }
     if(ctas == 1)
     {
         if(lane == 0) row_parts[warp] = part;
@@ -714,12 +728,17 @@ int launch_fwd_as(const void* logits, int64_t pitch, const float* tokens, float*
 //    8192 x 16000 fp32           20      116     113     105     150
 //    8192 x 32000 fp32           64              251     232     211
 //    8192 x 50021 bf16           64              244     199     222
-// Few rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read.
-int threads_of(int64_t vectors, int64_t top)
+// Where all rows run at once a row's latency is all there is, and more threads shorten it: 300 x 6000 fp32 with 20 alternatives
+// 8.0 us with 128 threads, 9.8 with 32; 300 x 16000 bf16 with 64 10.4, with 64 threads 18.5; rows of 88 vectors are better left to 32
+// threads.  Few long rows: a row is shared by the CTAs of a cluster, as long as each has two vectors per thread to read.
+int threads_of(int64_t rows, int64_t vectors, int64_t top)
 {
-    if(top == 0) return vectors <= 2048 ? 32 : 128;
-    if(top <= 24 && vectors <= 1024) return 32;
-    if(top <= 64 && vectors <= 2048) return 64;
+    if(rows > 4 * kSmCount || vectors < 256)
+    {
+        if(top == 0 && vectors <= 2048) return 32;
+        if(top > 0 && top <= 24 && vectors <= 1024) return 32;
+        if(top > 0 && top <= 64 && vectors <= (top <= 32 ? 2048 : 1024)) return 64;
+    }
     return top > 32 && vectors >= 7168 ? 256 : 128;
 }
 
@@ -731,7 +750,7 @@ int launch_fwd(const void* logits, int64_t pitch, const float* tokens, float* lo
     const int64_t vectors = V / Logit<DTYPE>::VE;
     int ctas = 1;
     while(ctas < kMaxCluster && rows * ctas * 2 <= 4 * kSmCount && vectors >= (int64_t)ctas * 1024) ctas *= 2;
-    const int T = ctas > 1 ? 256 : threads_of(vectors, top);
+    const int T = ctas > 1 ? 256 : threads_of(rows, vectors, top);
     const auto launch = top > 0 ? (T == 32 ? launch_fwd_as<DTYPE, true, 32> : T == 64 ? launch_fwd_as<DTYPE, true, 64> : T == 128 ? launch_fwd_as<DTYPE, true, 128> : launch_fwd_as<DTYPE, true, 256>)
                                 : (T == 32 ? launch_fwd_as<DTYPE, false, 32> : T == 128 ? launch_fwd_as<DTYPE, false, 128> : launch_fwd_as<DTYPE, false, 256>);
     return launch(logits, pitch, tokens, logprobs, entropy, lse, top_ids, top_logprobs, top, rows, V, c, inverse_temperature, ctas, stream);

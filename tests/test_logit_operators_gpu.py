@@ -866,3 +866,16 @@ def test_embedding_bwd_sorted_small_tables_of_repeated_ids(capi, two, accumulate
         want, size = want + before.double(), size + before.double().abs()
     # at most count + 4 roundings, each of at most half a step of a partial sum that the sum of the sizes bounds
     assert ((dW.double() - want).abs() <= (count + 4) * 2.0 ** -24 * size + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [6, 650])
+@pytest.mark.parametrize("V", [100, 130, 257, 300, 520, 700, 1000, 1030, 1300, 1600, 2050, 2600])
+def test_token_logprobs_long_lists_of_short_rows(capi, rows, V, dtype):
+    """Lists as long as a row has vectors or longer: the warps of a row have different numbers of vectors, some none."""
+    x = make_logits(rows, V, dtype, pitch=V + 3, offset=1, seed=V)
+    x[::5] = (x[::5] * 2).round() / 2
+    x[2::9, : V - V // 16] = -INF
+    tokens = make_tokens(rows, V)
+    for top in (3, 20, 24, 25, 33, 64, 65, 100, 128):
+        check_logprobs(capi, x, tokens, top, 1.0)
