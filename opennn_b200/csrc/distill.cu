@@ -7,7 +7,8 @@
 //
 // Bound by HBM at one read and one write of each logit: DRAM traffic is that (0.30 GB read for 0.30 GB of logits), the second
 // sweep comes from L1 (45 % of all loads) and L2.  Measured on a B200 (copy bandwidth 6.57 TB/s): 16384 x 32000 fp32 with both
-// parts at temperature 2, 37 % of the rows padding, 585 us = 5.8 TB/s; 4096 x 131072 bf16 with the soft part 419 us = 5.1 TB/s,
+// parts at temperature 2, 37 % of the rows padding, 577 us = 5.9 TB/s, 8192 x 32000 fp32 at temperature 1 341 us = 6.1 TB/s;
+// 4096 x 131072 bf16 with the soft part 388 us = 5.5 TB/s,
 // where the exponentials (two per logit, 16 per clock and SM) take 238 us by themselves.  Holding the row on chip instead was
 // slower: in the registers of a cluster of CTAs 789 and 776 us, in a persistent cluster with the next row's copies under way
 // 1163 and 1220 us (a cluster barrier and some 500 instructions per thread and row had nothing to hide behind).
@@ -188,7 +189,7 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
             if(id[k] < 0 || id[k] >= V) { id[k] = -1; u[k] = -INFINITY; }
             largest = fmaxf(largest, u[k]);
         }
-        largest = finite_anchor(warp_max(largest));
+        largest = finite_anchor(warp_largest(largest));
         float e[kPlaces], sum = 0.f;
 #pragma unroll
         for(int k = 0; k < kPlaces; k++)
@@ -210,7 +211,7 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
         }
         if(lane == 0) shared.taught = sum != 0.f;
     }
-    const float warp_m = warp_max(m);
+    const float warp_m = warp_largest(m);
     {
         const float down = m > -INFINITY ? m - finite_anchor(warp_m) : -INFINITY;
         s = warp_sum(s * exp2_approx(down * c));
@@ -219,7 +220,7 @@ distill3d_kernel(const typename Logit<DTYPE>::type* logits, long long pitch, con
     if(lane == 0) shared.parts[warp] = Part{warp_m, s, s1};
     __syncthreads();
     const Part other = lane < kWarpsHere ? shared.parts[lane] : Part{-INFINITY, 0.f, 0.f};
-    const float M = finite_anchor(warp_max(other.m));
+    const float M = finite_anchor(warp_largest(other.m));
     {
         const float down = other.m > -INFINITY ? other.m - M : -INFINITY;
         s = warp_sum(other.s * exp2_approx(down * c));

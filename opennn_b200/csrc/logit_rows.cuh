@@ -147,6 +147,14 @@ __device__ __forceinline__ float exp2_approx(float x)
     return y;
 }
 
+// The largest of the lanes' values in one instruction; NaN is passed by.
+__device__ __forceinline__ float warp_largest(float value)
+{
+    float t;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(t) : "f"(value));
+    return t;
+}
+
 // Two fp32 operations per instruction.
 __device__ __forceinline__ unsigned long long pair_bits(float2 v)
 {
