@@ -8,8 +8,8 @@
 // Bound by HBM at one read and one write of each logit: DRAM traffic is that (0.30 GB read for 0.30 GB of logits), the second
 // sweep comes from L1 (45 % of all loads) and L2.  Measured on a B200 (copy bandwidth 6.57 TB/s): 16384 x 32000 fp32 with both
 // parts at temperature 2, 37 % of the rows padding, 577 us = 5.9 TB/s, 8192 x 32000 fp32 at temperature 1 341 us = 6.1 TB/s;
-// 4096 x 131072 bf16 with the soft part 388 us = 5.5 TB/s,
-// where the exponentials (two per logit, 16 per clock and SM) take 238 us by themselves.  Holding the row on chip instead was
+// 4096 x 131072 bf16 with the soft part 388 us = 5.5 TB/s, where the exponentials (two per logit, 16 per clock and SM) take 238 us by
+// themselves (times of the kernel alone).  Holding the row on chip instead was
 // slower: in the registers of a cluster of CTAs 789 and 776 us, in a persistent cluster with the next row's copies under way
 // 1163 and 1220 us (a cluster barrier and some 500 instructions per thread and row had nothing to hide behind).
 #include <float.h>

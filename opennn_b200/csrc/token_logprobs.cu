@@ -332,7 +332,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     }
 
     // every warp's part to every CTA of the cluster
-    const float warp_m = warp_max(r.m);
+    const float warp_m = warp_largest(r.m);
     rebase(r, warp_m, c);
     Part part;
     part.m = warp_m;
@@ -374,7 +374,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         for(int i = lane; i < parts; i += 32) all = merge(all, Running{row_parts[i].m, row_parts[i].s, row_parts[i].w}, c);
         if(parts > 1)
         {
-            rebase(all, warp_max(all.m), c);
+            rebase(all, warp_largest(all.m), c);
             all.s = warp_sum(all.s);
             all.w = warp_sum(all.w);
         }
@@ -411,7 +411,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
         {
             float lowest = INFINITY;
             for(int i = lane; i < parts; i += 32) lowest = fminf(lowest, row_parts[i].top);
-            bound = -warp_max(-lowest);
+            bound = -warp_largest(-lowest);
         }
         bound = fmaxf(bound, -FLT_MAX);                // -inf is no alternative
 
@@ -546,7 +546,7 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             // no bound: the lowest candidate
             float lowest = INFINITY;
             for(int i = tid; i < n; i += T) lowest = fminf(lowest, key_logit(shared.candidates[i]));
-            lowest = -warp_max(-lowest);
+            lowest = -warp_largest(-lowest);
             if(lane == 0) row_parts[warp].m = lowest;
             __syncthreads();
             low = row_parts[0].m;
