@@ -193,7 +193,7 @@ int onn_embedding_bwd(const float* ids, const float* dY, const float* dY2, float
 
 /* The same gradient summed by token in a fixed order, for callers that want the same bits from every run:
  *   dW[v,:] = sqrt(E) (if scale) * sum over the positions with id v of (dY + dY2),  0 < v < V.
- * The order of the additions depends on B * S and the ids alone.  Nothing is added atomically, so frequent tokens do
+ * The order of the additions depends on the sizes and the ids alone (not on alignment or timing).  Nothing is added atomically, so frequent tokens do
  * not contend (onn_embedding_bwd adds each position's row with fp32 reductions in whatever order they arrive).
  * flags 0: all of dW [V, E] is overwritten, with zeros for row 0 and for tokens that do not occur; ONN_ACCUMULATE: added
  * to the rows of the tokens that do, the others are left alone.  E, V < 2^23, B * S < 2^31 - 65536.

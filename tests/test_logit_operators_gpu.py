@@ -879,3 +879,26 @@ def test_token_logprobs_long_lists_of_short_rows(capi, rows, V, dtype):
     tokens = make_tokens(rows, V)
     for top in (3, 20, 24, 25, 33, 64, 65, 100, 128):
         check_logprobs(capi, x, tokens, top, 1.0)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("E", [100004, 100001])
+def test_embedding_bwd_sorted_very_wide_rows(capi, E, accumulate):
+    """More column blocks than the kernel that joins runs has CTAs; one long run, several short ones."""
+    V, n = 40, 200
+    gen = generator(E)
+    ids = torch.randint(1, V, (1, n), generator=gen, device="cuda").float()
+    ids[0, 20:150] = 7.0
+    ids[0, 150:175] = 9.0
+    dY = torch.randn(1, n, E, generator=gen, device="cuda")
+    before = torch.randn(V, E, generator=gen, device="cuda")
+    dW = before.clone()
+    capi.embedding_bwd_sorted(ids, dY, V, dW=dW, accumulate=accumulate)
+    index = ids.view(-1).long()
+    want = torch.zeros(V, E, dtype=torch.float64, device="cuda").index_add_(0, index, dY[0].double()) * math.sqrt(E)
+    size = torch.zeros(V, E, dtype=torch.float64, device="cuda").index_add_(0, index, dY[0].double().abs()) * math.sqrt(E)
+    if accumulate:
+        want, size = want + before.double(), size + before.double().abs()
+    count = torch.bincount(index, minlength=V)[:, None]
+    # at most count + 3 roundings (with the scale's own and the earlier value's), each of at most half a step of a partial sum
+    assert ((dW.double() - want).abs() <= (count + 3) * 2.0 ** -24 * size).all()
