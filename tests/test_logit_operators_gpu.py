@@ -902,3 +902,16 @@ def test_embedding_bwd_sorted_very_wide_rows(capi, E, accumulate):
     count = torch.bincount(index, minlength=V)[:, None]
     # at most count + 3 roundings (with the scale's own and the earlier value's), each of at most half a step of a partial sum
     assert ((dW.double() - want).abs() <= (count + 3) * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("two", [False, True])
+def test_embedding_bwd_sorted_same_bits_at_any_alignment(capi, two):
+    B, S, E, V = 8, 600, 132, 900
+    gen = generator(5)
+    ids = torch.exp(torch.rand(B, S, generator=gen, device="cuda") * math.log(V)).floor().clamp(1, V - 1)
+    dY, dY2 = (torch.randn(B, S, E, generator=gen, device="cuda") for _ in range(2))
+    aligned = capi.embedding_bwd_sorted(ids, dY, V, dY2=dY2 if two else None)
+    room = torch.empty(dY.numel() + 1, device="cuda")
+    moved = room[1:].view(B, S, E)
+    moved.copy_(dY)
+    assert torch.equal(capi.embedding_bwd_sorted(ids, moved, V, dY2=dY2 if two else None), aligned)
