@@ -22,18 +22,19 @@ namespace
 {
 
 // Running statistics of a set of logits, in base 2 and relative to the largest logit m seen: with c = log2(e) / T,
-// a = c max(m, -kHuge) and d = c x - a in one rounding,  s = sum 2^d  and  w = sum 2^d d.  Every set with the
-// same m has the same a, so its rounding shifts all terms alike and is taken out at the end.  -inf adds nothing to either
-// sum; NaN and +inf make both NaN.  Logits below -kHuge count as nothing, and beyond |m| = kHuge c x could overflow: a row
-// whose largest logit is that far out is summed again (huge_row).
+// a = max(c m, -kFar) and d = c x - a in one rounding,  s = sum 2^d  and  w = sum 2^d d.  Every set with the
+// same m has the same a, so its rounding shifts all terms alike and is taken out at the end.  That shift is up to half a step of c m
+// (the d of the largest logit itself): within kFar at most 8, which costs the entropy a few bits; at 2^31 it is 64, and a little
+// later 2^d overflows.  So a set of nothing but logits below -kFar (a finite mask) adds nothing when it meets a larger one, and a row
+// whose largest logit is beyond +-kFar is summed again (far_row).  -inf adds nothing to either sum; NaN and +inf make both NaN.
 struct Running { float m, s, w; };
 
 constexpr float kNothing = -1e4f;                 // 2^-10000 = 0: the bound that keeps 0 * -inf out of w
-constexpr float kHuge = 1e29f;
+constexpr float kFar = 268435456.f;               // 2^28
 
 __device__ __forceinline__ float finite_anchor(float m) { return m > -INFINITY ? m : 0.f; }
 // rounded once, whatever it is subtracted from (no contraction into a fused multiply-add)
-__device__ __forceinline__ float anchor(float m, float c) { return __fmul_rn(fmaxf(m, -kHuge), c); }
+__device__ __forceinline__ float anchor(float m, float c) { return fmaxf(__fmul_rn(m, c), -kFar); }
 
 // The sums of r relative to another, larger m.
 __device__ __forceinline__ void rebase(Running& r, float m, float c)
@@ -84,19 +85,30 @@ __device__ __forceinline__ void add_vectors(Running& r, const uint4 (&v)[N], flo
     r.w += w2.x + w2.y;
 }
 
-// The sums of a whole row by one warp, with the difference taken before the scale: right for logits of any finite size
-// (nothing but a mask of the type's lowest value), and rare.
+// The sums of a whole row by one warp, with the difference taken before the scale: right for logits of any finite size,
+// and rare (a row of nothing but a finite mask, large logits at a temperature near zero).
 template <int DTYPE>
-__device__ __noinline__ Running huge_row(const typename Logit<DTYPE>::type* x, int V, float m, float c)
+__device__ __noinline__ Running far_row(const typename Logit<DTYPE>::type* x, int V, float m, float c)
 {
-    Running r = {m, 0.f, 0.f};
-    for(int i = threadIdx.x & 31; i < V; i += 32)
+    // eight loads of a lane under way, and eight short sums instead of a long one
+    constexpr int N = 8;
+    float s[N] = {}, w[N] = {};
+    for(int start = threadIdx.x & 31; start < V; start += N * 32)
     {
-        const float d = (Logit<DTYPE>::get(x + i) - m) * c;
-        const float p = exp2_approx(d);
-        r.s += p;
-        r.w = fmaf(p, fmaxf(d, kNothing), r.w);
+        float d[N];
+#pragma unroll
+        for(int u = 0; u < N; u++) d[u] = start + u * 32 < V ? (Logit<DTYPE>::get(x + start + u * 32) - m) * c : -INFINITY;
+#pragma unroll
+        for(int u = 0; u < N; u++)
+        {
+            const float p = exp2_approx(d[u]);
+            s[u] += p;
+            w[u] = fmaf(p, fmaxf(d[u], kNothing), w[u]);
+        }
     }
+    Running r = {m, 0.f, 0.f};
+#pragma unroll
+    for(int u = 0; u < N; u++) { r.s += s[u]; r.w += w[u]; }
     r.s = warp_sum(r.s);
     r.w = warp_sum(r.w);
     return r;
@@ -379,14 +391,14 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
             all.w = warp_sum(all.w);
         }
         else all = Running{part.m, part.s, part.w};
-        const bool huge = fabsf(all.m) >= kHuge && fabsf(all.m) < INFINITY;
-        if(huge) all = huge_row<DTYPE>(x, V, all.m, c);
+        const bool far = fabsf(all.m * c) >= kFar && fabsf(all.m) < INFINITY;
+        if(far) all = far_row<DTYPE>(x, V, all.m, c);
         if(lane == 0)
         {
             const bool none = all.s == 0.f;            // a row without a finite logit has no distribution
             const float log_2s = logf(all.s);
             // relative to m itself: the rounding of the anchor
-            const float log_s = none ? INFINITY : huge ? log_2s : fmaf(fmaf(all.m, c, -anchor(all.m, c)), -kLn2, log_2s);
+            const float log_s = none ? INFINITY : far ? log_2s : fmaf(fmaf(all.m, c, -anchor(all.m, c)), -kLn2, log_2s);
             if constexpr(TOP) { shared.m = finite_anchor(all.m); shared.log_s = log_s; }
             if(logprobs) logprobs[row] = none ? -INFINITY : (given - all.m) * inverse_temperature - log_s;
             if(entropy)
