@@ -417,7 +417,9 @@ int onn_token_logprobs(const void* logits, int dtype, int64_t pitch, const float
  * gradients of the two outputs, d_logprobs [rows] and d_entropy [rows] (NULL: no gradient through the entropy; entropy
  * may then be NULL too),
  *   dlogits_i = (d_logprob (1[i = token] - p_i) - d_entropy p_i (log p_i + entropy)) / temperature,
- * 0 on padding rows, rounded once to dtype.  dlogits (row r at dlogits + r * d_pitch elements) is overwritten; it may
+ * 0 on padding rows, rounded once to dtype.  p = exp(z - lse) with lse as given; where |lse| >= 16384 (a row of nothing but a finite
+ * mask, large logits at a small temperature) its rounding to fp32 would show in p, which is then formed from the row's
+ * largest logit and sum, at the price of two more reads of the row.  dlogits (row r at dlogits + r * d_pitch elements) is overwritten; it may
  * be the logits themselves (with the same pitch, another is refused), but must not overlap them in another way.  Elements between V and the pitch
  * are left as they are. */
 int onn_token_logprobs_bwd(const void* logits, int dtype, int64_t pitch, const float* tokens, const float* lse,

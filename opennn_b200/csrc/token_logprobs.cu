@@ -617,6 +617,41 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
     if(!met) asm volatile("barrier.cluster.wait;" ::: "memory");
 }
 
+// exp(z - lse) carries the rounding of lse: half a step of it is at most 2^-11 below this bound, and p is anything once it exceeds 1.
+constexpr float kFarLse = 16384.f;
+
+// The gradient of a row whose log-sum-exp is that far out (a row of nothing but a finite mask, large logits at a temperature near zero,
+// nothing but -inf), by one CTA: the largest logit and the sum relative to it first, then p from the difference.  Rare.
+template <int DTYPE, bool ENTROPY, int T>
+__device__ __noinline__ void far_gradient(const typename Logit<DTYPE>::type* x, typename Logit<DTYPE>::type* dx, int V, int token, float g, float h, float H,
+                                          float inverse_temperature)
+{
+    using L = Logit<DTYPE>;
+    __shared__ float scratch[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float m = -INFINITY;
+    for(int i = tid; i < V; i += T) m = fmaxf(m, L::get(x + i));      // no NaN: lse would be NaN too
+    m = warp_largest(m);
+    if(lane == 0) scratch[warp] = m;
+    __syncthreads();
+    m = scratch[0];
+#pragma unroll
+    for(int w = 1; w < T / 32; w++) m = fmaxf(m, scratch[w]);
+    m = finite_anchor(m);
+    const float c = kLog2E * inverse_temperature;
+    float s = 0.f;
+    for(int i = tid; i < V; i += T) s += exp2_approx((L::get(x + i) - m) * c);
+    s = block_sum(s, scratch);
+    const float log_s = s == 0.f ? 0.f : logf(s);       // no finite logit: every p is 0
+    for(int i = tid; i < V; i += T)
+    {
+        const float log_p = fmaf(L::get(x + i) - m, inverse_temperature, -log_s), p = exp2_approx(log_p * kLog2E);
+        float value = -g * p;
+        if(ENTROPY) value = fmaf(-h, fmaxf(log_p, kNothing) + H, -g) * p;
+        L::put(dx + i, value + (i == token ? g : 0.f));
+    }
+}
+
 // One CTA per piece of a row: the row's scalars, then batches of vectors: load, compute, store.
 template <int DTYPE, bool ENTROPY, int T, int N>
 __global__ void __launch_bounds__(T, 1024 / T)
@@ -646,8 +681,13 @@ token_logprobs_bwd_kernel(const typename Logit<DTYPE>::type* logits, long long p
     const float g = d_logprobs[row] * inverse_temperature;
     const float h = ENTROPY ? d_entropy[row] * inverse_temperature : 0.f;
     const float H = ENTROPY ? entropy[row] : 0.f;
-    float row_lse = lse[row];
-    if(row_lse == -INFINITY) row_lse = 0.f;            // a row without a finite logit: every p is 0
+    const float row_lse = lse[row];
+    if(fabsf(row_lse) >= kFarLse)
+    {
+        // all by one CTA: where the gradient takes the logits' place nobody else may write while it reads
+        if(blockIdx.x == 0) far_gradient<DTYPE, ENTROPY, T>(x, dx, V, (int)token, g, h, H, inverse_temperature);
+        return;
+    }
     const float2 minus_lse = make_float2(-row_lse, -row_lse), it2 = make_float2(inverse_temperature, inverse_temperature);
     const float2 log2e2 = make_float2(kLog2E, kLog2E), minus_g = make_float2(-g, -g), minus_h = make_float2(-h, -h), H2 = make_float2(H, H);
     auto two = [&](float2 value)
