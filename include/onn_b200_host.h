@@ -104,7 +104,8 @@ int onn_trainer_forward(onn_trainer* trainer, const float* decoder_ids, const fl
  * onn_token_logprobs on the output layer's logits.  targets [micro_batch, decoder_sequence_length] (NULL: no logprobs, every
  * position takes part); logprobs, entropy [rows] and top_ids, top_logprobs [rows, top] as in onn_token_logprobs, with
  * rows = micro_batch * decoder_sequence_length; NULL for what is not wanted.  All are device pointers; the work runs on
- * onn_trainer_stream() and is not waited for. */
+ * onn_trainer_stream() and is not waited for.  The output layer is left with the logits, as after a training pass:
+ * onn_trainer_get_layer_output reads logits there until the next onn_trainer_forward with is_training = 0 or decoding. */
 int onn_trainer_token_logprobs(onn_trainer* trainer, const float* decoder_ids, const float* encoder_ids, const float* targets,
                                float temperature, float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, int64_t top);
 /* Greedy decoding on token ids: the loop of Transformer::calculate_outputs (opennn/standard_networks.cpp:1002-1035)

@@ -167,7 +167,8 @@ class Trainer:
 
     def token_logprobs(self, dec_ids, enc_ids, targets=None, top=0, temperature=1.0):
         """Scores targets under the network.  dec_ids, enc_ids, targets: torch CUDA float tensors of one micro-batch.  Returns
-        (logprobs, entropy [micro_batch, S_dec], top_ids, top_logprobs [micro_batch, S_dec, top]), None for what is not asked."""
+        (logprobs, entropy [micro_batch, S_dec], top_ids, top_logprobs [micro_batch, S_dec, top]), None for what is not asked.
+        The output layer holds logits afterwards (layer_output), where forward(is_training=False) leaves probabilities."""
         import torch
         shape = (self.micro_batch, self.S_dec)
         if tuple(dec_ids.shape) != shape or (targets is not None and tuple(targets.shape) != shape):
