@@ -24,13 +24,13 @@ namespace
 // Running statistics of a set of logits, in base 2 and relative to the largest logit m seen: with c = log2(e) / T,
 // a = max(c m, -kFar) and d = c x - a in one rounding,  s = sum 2^d  and  w = sum 2^d d.  Every set with the
 // same m has the same a, so its rounding shifts all terms alike and is taken out at the end.  That shift is up to half a step of c m
-// (the d of the largest logit itself): within kFar at most 8, which costs the entropy a few bits; at 2^31 it is 64, and a little
-// later 2^d overflows.  So a set of nothing but logits below -kFar (a finite mask) adds nothing when it meets a larger one, and a row
-// whose largest logit is beyond +-kFar is summed again (far_row).  -inf adds nothing to either sum; NaN and +inf make both NaN.
+// (the d of the largest logit itself): within kFar at most 64, a little later 2^d overflows.  So a set of nothing but logits below
+// -kFar / c (a finite mask) adds nothing when it meets a larger one, and a row whose largest logit is beyond +-kFar / c is summed again
+// (far_row).  -inf adds nothing to either sum; NaN and +inf make both NaN.
 struct Running { float m, s, w; };
 
 constexpr float kNothing = -1e4f;                 // 2^-10000 = 0: the bound that keeps 0 * -inf out of w
-constexpr float kFar = 268435456.f;               // 2^28
+constexpr float kFar = 2147483648.f;              // 2^31
 
 __device__ __forceinline__ float finite_anchor(float m) { return m > -INFINITY ? m : 0.f; }
 // rounded once, whatever it is subtracted from (no contraction into a fused multiply-add)
@@ -86,7 +86,8 @@ __device__ __forceinline__ void add_vectors(Running& r, const uint4 (&v)[N], flo
 }
 
 // The sums of a whole row by one warp, with the difference taken before the scale: right for logits of any finite size,
-// and rare (a row of nothing but a finite mask, large logits at a temperature near zero).
+// and rare (a row of nothing but a mask far out, large logits at a temperature near zero).  16384 x 32000 fp32 with every row of that kind
+// 1048 us, ordinary 298; one row of 131072 197 us, ordinary 10.
 template <int DTYPE>
 __device__ __noinline__ Running far_row(const typename Logit<DTYPE>::type* x, int V, float m, float c)
 {
