@@ -621,8 +621,9 @@ token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, lo
 // exp(z - lse) carries the rounding of lse: half a step of it is at most 2^-11 below this bound, and p is anything once it exceeds 1.
 constexpr float kFarLse = 16384.f;
 
-// The gradient of a row whose log-sum-exp is that far out (a row of nothing but a finite mask, large logits at a temperature near zero,
-// nothing but -inf), by one CTA: the largest logit and the sum relative to it first, then p from the difference.  Rare.
+// The gradient of a row whose log-sum-exp is that far out (a row of nothing but a finite mask, large logits at a temperature near zero),
+// by one CTA: the largest logit and the sum relative to it first, then p from the difference.  Rare: 16384 x 32000 fp32 with every
+// row of that kind 1490 us, ordinary 648; one row of 131072 114 us, ordinary 12.
 template <int DTYPE, bool ENTROPY, int T>
 __device__ __noinline__ void far_gradient(const typename Logit<DTYPE>::type* x, typename Logit<DTYPE>::type* dx, int V, int token, float g, float h, float H,
                                           float inverse_temperature)
@@ -682,7 +683,9 @@ token_logprobs_bwd_kernel(const typename Logit<DTYPE>::type* logits, long long p
     const float g = d_logprobs[row] * inverse_temperature;
     const float h = ENTROPY ? d_entropy[row] * inverse_temperature : 0.f;
     const float H = ENTROPY ? entropy[row] : 0.f;
-    const float row_lse = lse[row];
+    float row_lse = lse[row];
+    // a row without a finite logit: every p is 0.  Below temperature 1 -inf may also be a finite z past fp32.
+    if(row_lse == -INFINITY && inverse_temperature <= 1.f) row_lse = 0.f;
     if(fabsf(row_lse) >= kFarLse)
     {
         // all by one CTA: where the gradient takes the logits' place nobody else may write while it reads

@@ -194,3 +194,21 @@ def test_token_logprobs_bwd_log_sum_past_fp32(capi):
         # H and log p, each of size log V, cancel but for their roundings
         tol = (g.abs().double()[:, None] * p * (chain(V) + 8 * U) + h.abs().double()[:, None] * p * 4 * (chain(V) + 8 * U) * (1 + math.log(V))) / T + 4 * U * want.abs()
         check_close(dx, want, tol, "dlogits")
+
+
+@pytest.mark.parametrize("T", [0.25, 1.0, 2.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_token_logprobs_bwd_rows_without_a_finite_logit(capi, dtype, T):
+    """p = 0 throughout: the gradient is the token's alone.  Powers of two: no rounding at all."""
+    for V in (33, 40000):
+        x = torch.full((3, V), -INF, dtype=TYPES[dtype], device="cuda")
+        tokens = torch.tensor([1.0, 0.0, V - 1.0], device="cuda")
+        g, h = torch.tensor([0.5, 0.25, -2.0], device="cuda"), torch.ones(3, device="cuda")
+        _, H, lse, _, _ = capi.token_logprobs(x, tokens, temperature=T)
+        assert lse[0] == -INF and lse[2] == -INF
+        want = torch.zeros(3, V, dtype=x.dtype, device="cuda")
+        want[0, 1], want[2, V - 1] = 0.5 / T, -2.0 / T
+        for entropy in (None, h):
+            assert torch.equal(capi.token_logprobs_bwd(x, tokens, lse, H, g, entropy, temperature=T), want)
+        capi.token_logprobs_bwd(x, tokens, lse, H, g, h, temperature=T, out=x)
+        assert torch.equal(x, want)
