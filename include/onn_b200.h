@@ -408,7 +408,8 @@ int onn_ce3d_fwd_bwd(float* logits, const float* targets, const float* active_co
  * Logits of -inf (masked tokens) have probability 0 and never stand in the list; places left over hold -1 and -inf.
  * A row of nothing but -inf receives -inf, 0, -inf and an empty list.  A row that holds NaN or +inf receives NaN
  * for logprob, entropy and lse and in the values of its list (NaN logits are not listed).
- * temperature is in [1e-6, 1e6]; rows < 2^27.
+ * Finite masks (-1e9 and the like) are logits as any other: a row of nothing but one value has entropy log V.
+ * temperature is in [1e-6, 1e6]; rows < 2^27; 2 <= V < 2^31 - 4096.
  * ------------------------------------------------------------------------------------- */
 int onn_token_logprobs(const void* logits, int dtype, int64_t pitch, const float* tokens,
                        float* logprobs, float* entropy, float* lse, int32_t* top_ids, float* top_logprobs, int64_t top,

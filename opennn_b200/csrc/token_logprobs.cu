@@ -5,9 +5,12 @@
 //   backward  dx_i = [ g (1[i = t] - p_i) - h p_i (log p_i + entropy) ] / T
 //
 // Both are bound by HBM: the forward pass reads each logit once, the backward pass reads and writes each once.  Measured on a
-// B200 (copy bandwidth 6.57 TB/s): forward without a list 16384 x 32000 fp32 191 to 199 us = 6.6 to 6.9 TB/s, 8192 x 50021
-// bf16 141 us = 5.8 TB/s; with 64 alternatives 189 us = 4.3 TB/s: there the instructions bound it (12 to 13 per logit,
-// 70 % of the issue slots), the exponential and the two sums taking most of them.  Backward 8192 x 32000 fp32 with entropy 267 us = 6.4 TB/s.
+// B200 (copy bandwidth 6.57 TB/s): forward without a list 16384 x 32000 fp32 298 us = 7.0 TB/s, with 37 % of the rows padding, which
+// are not read (1.31 GB), 195 to 202 us = 6.5 to 6.7 TB/s, 8192 x 50021 bf16 142 us = 5.8 TB/s; with 64 alternatives 189 us = 4.3 TB/s:
+// there the instructions bound it (12 to 13 per logit, 70 % of the issue slots; about five are the sums' own: two for unpacking, one to
+// floor, a multiply-add, two exponentials and two sums for a pair, and its share of the maximum; the rest, batches ahead, unit maxima, the
+// second reading and the ranking, is not told apart).  Backward 8192 x 32000 fp32 with entropy, padded in the same way, 262 to 278 us
+// = 6.1 to 6.5 TB/s.
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -187,8 +190,9 @@ struct Shared<true, T>
 // batches of a long row).  If every warp knows k logits that are at least t, with k = ceil(top / warps), no logit below t can
 // stand in the list; so the k-th largest of the lanes' two best units is the warp's bound, and the smallest bound of all warps
 // the row's.  Only units that reach it (little more than `top` of them) are read again, most often from L2, and
-// their logits that reach it become candidates in the first CTA, which ranks them.  Should a thousand logits reach
-// the bound (equal ones), the row is scanned once for each place.
+// their logits that reach it become candidates in the first CTA, which ranks them.  Should more logits reach the bound than the list of
+// candidates holds, the row is scanned once for each place: equal ones, or a neighbouring stretch so unlikely (masked) that a warp has to
+// vouch with it for more places than it has better logits.  Then one row of 131072 bf16 with 64 alternatives takes 1483 us instead of 10.
 template <int DTYPE, bool TOP, int T, int N>
 __global__ void __launch_bounds__(T, T == 32 ? 24 : 1024 / T)
 token_logprobs_kernel(const typename Logit<DTYPE>::type* __restrict__ logits, long long pitch, const float* __restrict__ tokens,
